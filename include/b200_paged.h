@@ -60,7 +60,8 @@ enum b2p_device_error {
   B2P_DEV_SLOT_RANGE = 1,   /* slot id >= num_slots                      */
   B2P_DEV_BLOCK_RANGE = 2,  /* block id outside [0, num_slots/block_size) */
   B2P_DEV_WAIT_TIMEOUT = 4, /* a bounded mbarrier / flag wait gave up     */
-  B2P_DEV_LENGTH = 8        /* a context/query length that does not fit  */
+  B2P_DEV_LENGTH = 8,       /* a context/query length that does not fit  */
+  B2P_DEV_TOKEN_RANGE = 16  /* drafted token id outside the vocabulary   */
 };
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -286,6 +287,136 @@ B2P_API int b2p_lm_head_argmax(const void* hidden, int64_t hidden_row_stride, co
                                int hidden_size, int dtype, int64_t* out_ids, float* out_max,
                                void* workspace, size_t workspace_bytes, int32_t* err_flag,
                                void* stream);
+
+/*
+ * The 8-bit KV cache (no counterpart in the reference, which stores the model's dtype).
+ *   key_cache, value_cache   : e4m3 codes [num_layers, num_slots, num_kv_heads, head_dim]
+ *   key_scales, value_scales : fp32 [num_layers, num_slots / block_size, num_kv_heads]
+ * An element stands for code * scale of its (layer, block, head). The write below keeps every
+ * scale a power of two: 2^e with the smallest e >= -110 for which the block's largest magnitude
+ * is at most 448 * 2^e. A NaN or an infinity among a block's rows makes its scale NaN until the
+ * block is started anew. Readers take any scale.
+ *
+ * K7 -- b2p_kv_write_fp8: sequence i appends rows [cu_seqlens_q[i], cu_seqlens_q[i+1]) of
+ * keys/values (bf16, f16 or fp32; strides in elements) at positions context_lens[i] - q_len_i ..
+ * context_lens[i] - 1, through its block table. A write that covers a block's first slot starts
+ * the block anew: what its other slots held before is dropped. Any other write keeps the larger of
+ * the block's scale and the one its rows need, and rounds the codes before its first row to it.
+ *   max_q_len : upper bound of the q_len_i; a longer one, or one above its context, is skipped
+ *               and sets B2P_DEV_LENGTH. A block id outside the pool sets B2P_DEV_BLOCK_RANGE.
+ * Two sequences of one call must not append to the same block (copy it first,
+ * b2p_copy_blocks): which of them it then holds is not specified. head_dim % 8 == 0.
+ */
+B2P_API int b2p_kv_write_fp8(const void* keys, int64_t k_tok_stride, int64_t k_head_stride,
+                 const void* values, int64_t v_tok_stride, int64_t v_head_stride,
+                 void* key_cache, void* value_cache, float* key_scales, float* value_scales,
+                 const int32_t* block_tables, int64_t block_table_stride,
+                 const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
+                 int64_t num_rows, int max_q_len, int64_t layer_index, int64_t num_layers,
+                 int64_t num_slots, int num_kv_heads, int head_dim, int block_size, int dtype,
+                 int32_t* err_flag, void* stream);
+
+/*
+ * Rows of the given slots as values of `dtype`: keys, values [num_rows, num_kv_heads, head_dim],
+ * contiguous. A negative slot gives zeros; one past the pool too, and sets B2P_DEV_SLOT_RANGE.
+ */
+B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, const float* key_scales,
+                 const float* value_scales, const int32_t* slot_mapping, int64_t num_rows,
+                 void* keys, void* values, int64_t layer_index, int64_t num_layers,
+                 int64_t num_slots, int num_kv_heads, int head_dim, int block_size, int dtype,
+                 int32_t* err_flag, void* stream);
+
+/*
+ * Attention over the 8-bit cache. Arguments as in b2p_paged_decode and b2p_paged_prefill; dtype is
+ * that of q and out. Rows without a key to see (context 0) are zeros and set B2P_DEV_LENGTH.
+ *   workspace : b2p_paged_fp8_workspace_size() bytes, zero before its first use with these heads
+ *               and zeroed again after B2P_DEV_WAIT_TIMEOUT; every completed call leaves it
+ *               usable for the next one on the stream. Calls that may overlap need one each.
+ *   max_q_len : upper bound of the q_len_i; rows of a longer sequence set B2P_DEV_LENGTH.
+ */
+B2P_API size_t b2p_paged_fp8_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads,
+                                            int head_dim, int max_q_len);
+B2P_API int b2p_paged_decode_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                 const void* key_cache, const void* value_cache, const float* key_scales,
+                 const float* value_scales, int64_t layer_index, int64_t num_layers,
+                 int64_t num_slots, const int32_t* block_tables, int64_t block_table_stride,
+                 const int32_t* context_lens, int num_seqs, int num_q_heads, int num_kv_heads,
+                 int head_dim, int block_size, float scale, void* out, int64_t out_tok_stride,
+                 int64_t out_head_stride, void* workspace, size_t workspace_size, int dtype,
+                 int32_t* err_flag, void* stream);
+B2P_API int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                 const void* key_cache, const void* value_cache, const float* key_scales,
+                 const float* value_scales, int64_t layer_index, int64_t num_layers,
+                 int64_t num_slots, const int32_t* block_tables, int64_t block_table_stride,
+                 const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
+                 int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
+                 int block_size, float scale, void* out, int64_t out_tok_stride,
+                 int64_t out_head_stride, void* workspace, size_t workspace_size, int dtype,
+                 int32_t* err_flag, void* stream);
+
+/*
+ * K8 -- verification of drafted tokens. Sequence i drafted tokens draft_tokens[cu_drafts[i] ..
+ * cu_drafts[i+1]) and owns the k_i + 1 target rows that start at row cu_drafts[i] + i.
+ * Draft j is accepted while accept_draws[j] * q_j(x_j) < p_j(x_j); with n accepted, one more token
+ * is the first index where the running sum of r exceeds sample_draws[i] * sum(r): r = max(p - q, 0)
+ * of row n after a rejection (p where that is zero everywhere), p of the last row otherwise.
+ *   target_probs : [total_drafts + num_seqs, vocab], draft_probs : [total_drafts, vocab] or NULL
+ *                  (q_j is then 1 at x_j), both of `dtype`, row strides in elements
+ *   draws        : fp32 in [0, 1)
+ *   out_tokens   : int64 [num_seqs, max_drafts + 1]: the accepted drafts, the drawn token, then -1
+ *   out_accepted : int32 [num_seqs]
+ * Sums are fp64. Negative and NaN probabilities count as zero; a row without a positive entry
+ * gives token 0. A drafted id outside the vocabulary is rejected and sets B2P_DEV_TOKEN_RANGE. A
+ * sequence with more than max_drafts drafts (or bad offsets) gets -1 everywhere and sets
+ * B2P_DEV_LENGTH.
+ */
+B2P_API int b2p_verify_drafts(const void* target_probs, int64_t target_row_stride,
+                 const void* draft_probs, int64_t draft_row_stride, const int64_t* draft_tokens,
+                 const int32_t* cu_drafts, const float* accept_draws, const float* sample_draws,
+                 int num_seqs, int64_t total_drafts, int max_drafts, int vocab, int dtype,
+                 int64_t* out_tokens, int64_t out_row_stride, int32_t* out_accepted,
+                 int32_t* err_flag, void* stream);
+
+/*
+ * The greedy form: target_ids [total_drafts + num_seqs] holds each target row's arg-max (what
+ * b2p_lm_head_argmax gives); a draft stands while it equals its row's id.
+ */
+B2P_API int b2p_verify_drafts_greedy(const int64_t* target_ids, const int64_t* draft_tokens,
+                 const int32_t* cu_drafts, int num_seqs, int64_t total_drafts, int max_drafts,
+                 int64_t* out_tokens, int64_t out_row_stride, int32_t* out_accepted,
+                 int32_t* err_flag, void* stream);
+
+/*
+ * K9 -- moves of pages (blocks), all layers of K and V in one call. element_bytes is 4, 2 or 1;
+ * key_scales and value_scales are those of an 8-bit pool, or both NULL.
+ *
+ * b2p_copy_blocks: block src_blocks[i] to block dst_blocks[i]; a pair with a negative id is
+ * skipped, one with an id past the pool too, and sets B2P_DEV_BLOCK_RANGE. Targets must be distinct
+ * and none of them a source of the same call: what such blocks hold afterwards is not specified.
+ */
+B2P_API int b2p_copy_blocks(void* key_cache, void* value_cache, float* key_scales,
+                 float* value_scales, const int32_t* src_blocks, const int32_t* dst_blocks,
+                 int64_t num_pairs, int64_t num_layers, int64_t num_slots, int num_kv_heads,
+                 int head_dim, int element_bytes, int block_size, int32_t* err_flag, void* stream);
+
+/*
+ * b2p_compact_blocks: moves the live blocks (those in the first ceil(context_lens[i] / block_size)
+ * entries of row i of block_tables) into the first num_live blocks of the pool and rewrites the
+ * tables in place. Live blocks already there stay; the j-th of the others, in ascending order, goes
+ * to the j-th free block. Blocks past num_live keep their bytes.
+ *   new_ids  : int32 [num_blocks], the new id of each live block, -1 for the others
+ *   num_live : int32 [1]
+ *   workspace: b2p_compact_blocks_workspace_size(num_blocks) bytes, any contents
+ * Bad table entries are left as they are and set B2P_DEV_BLOCK_RANGE; a context longer than its
+ * table row sets B2P_DEV_LENGTH.
+ */
+B2P_API size_t b2p_compact_blocks_workspace_size(int64_t num_blocks);
+B2P_API int b2p_compact_blocks(void* key_cache, void* value_cache, float* key_scales,
+                 float* value_scales, int32_t* block_tables, int64_t block_table_stride,
+                 int table_width, const int32_t* context_lens, int num_seqs, int64_t num_layers,
+                 int64_t num_slots, int num_kv_heads, int head_dim, int element_bytes,
+                 int block_size, int32_t* new_ids, int32_t* num_live, void* workspace,
+                 size_t workspace_size, int32_t* err_flag, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,7 @@ DEV_SLOT_RANGE = 1
 DEV_BLOCK_RANGE = 2
 DEV_WAIT_TIMEOUT = 4
 DEV_LENGTH = 8
+DEV_TOKEN_RANGE = 16
 
 EXPORTED_SYMBOLS = (
     "b2p_version",
@@ -44,6 +45,16 @@ EXPORTED_SYMBOLS = (
     "b2p_build_metadata",
     "b2p_lm_head_argmax_workspace_size",
     "b2p_lm_head_argmax",
+    "b2p_kv_write_fp8",
+    "b2p_kv_read_fp8",
+    "b2p_paged_fp8_workspace_size",
+    "b2p_paged_decode_fp8",
+    "b2p_paged_prefill_fp8",
+    "b2p_verify_drafts",
+    "b2p_verify_drafts_greedy",
+    "b2p_copy_blocks",
+    "b2p_compact_blocks_workspace_size",
+    "b2p_compact_blocks",
 )
 
 _lock = threading.Lock()
@@ -95,6 +106,43 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "b2p_lm_head_argmax": (
         _i32,
         [_p, _i64, _p, _i64, _i32, _i64, _i32, _i32, _p, _p, _p, _sz, _p, _p],
+    ),
+    "b2p_kv_write_fp8": (
+        _i32,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _p, _i32, _i64, _i32, _i64,
+         _i64, _i64, _i32, _i32, _i32, _i32, _p, _p],
+    ),
+    "b2p_kv_read_fp8": (
+        _i32,
+        [_p, _p, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p],
+    ),
+    "b2p_paged_fp8_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "b2p_paged_decode_fp8": (
+        _i32,
+        [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _i32, _i32, _i32, _i32,
+         _i32, _f32, _p, _i64, _i64, _p, _sz, _i32, _p, _p],
+    ),
+    "b2p_paged_prefill_fp8": (
+        _i32,
+        [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _i32, _i64, _i32,
+         _i32, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _sz, _i32, _p, _p],
+    ),
+    "b2p_verify_drafts": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _p, _p, _p, _i32, _i64, _i32, _i32, _i32, _p, _i64, _p, _p, _p],
+    ),
+    "b2p_verify_drafts_greedy": (
+        _i32, [_p, _p, _p, _i32, _i64, _i32, _p, _i64, _p, _p, _p],
+    ),
+    "b2p_copy_blocks": (
+        _i32,
+        [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p],
+    ),
+    "b2p_compact_blocks_workspace_size": (_sz, [_i64]),
+    "b2p_compact_blocks": (
+        _i32,
+        [_p, _p, _p, _p, _p, _i64, _i32, _p, _i32, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p,
+         _p, _sz, _p, _p],
     ),
 }
 

@@ -1,0 +1,341 @@
+// K8 — verification of drafted tokens (speculative decoding).
+//
+// Sequence i drafted k_i tokens x_0 .. x_{k-1}; row j of its k_i + 1 target rows is the target
+// model's distribution p_j for the token after x_{j-1}, and q_j is the distribution x_j was
+// drafted from. Draft j is accepted while u_j * q_j(x_j) < p_j(x_j). Then one more token is
+// drawn with v: with n accepted, the first index where the running sum of r exceeds v * sum(r),
+//   r = max(p_n - q_n, 0) after a rejection (p_n itself where that is zero everywhere),
+//   r = p_k               with all k accepted.
+// Without draft probabilities the draft is certain: q_j is 1 at x_j and 0 elsewhere. The token
+// stream this gives is distributed as the target model's own.
+//
+// Bytes: a handful of gathered values, then one row pair (p_n, q_n) per sequence, read once;
+// everything else is latency. One cluster of kCluster CTAs owns a sequence: every CTA takes a
+// slice of the vocabulary and every warp a contiguous piece of the slice; the piece sums meet
+// in distributed shared memory, and only the one piece that holds the crossing is read again
+// (from L2) to find the index. All sums are fp64 in a fixed order: p - q and u * q of fp32
+// inputs are exact there, and a token's interval is as narrow as its probability, so fp32
+// sums over 150,000 entries would move draws across the borders of rare tokens.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+using namespace b2p;
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kCluster = 8;
+
+struct VerifyParams {
+  const uint8_t* target;  // [total + num_seqs, vocab]
+  int64_t t_row;          // element strides
+  const uint8_t* draft;   // [total, vocab] or null
+  int64_t d_row;
+  const int64_t* tokens;  // [total]
+  const int32_t* cu;      // [num_seqs + 1]
+  const float* accept;    // [total]
+  const float* sample;    // [num_seqs]
+  int64_t total;
+  int num_seqs, max_drafts, vocab;
+  int64_t* out;  // [num_seqs, max_drafts + 1]
+  int64_t out_row;
+  int32_t* accepted;
+  int32_t* err;
+};
+
+// What a CTA needs to know of its sequence.
+struct Row {
+  int begin, k, n;   // first draft, drafts, accepted
+  int64_t rejected;  // the rejected token, -1: none (or out of range)
+};
+
+__device__ __forceinline__ double positive(double x) { return x > 0.0 ? x : 0.0; }  // NaN: 0
+
+template <typename T>
+__device__ __forceinline__ double residual(const T* p, const T* q, int64_t drop, int v) {
+  const double x = (double)to_f32<T>(p[v]);
+  if (q != nullptr) return positive(x - (double)to_f32<T>(q[v]));
+  return v == drop ? 0.0 : positive(x);
+}
+
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_drafts(const VerifyParams p) {
+  __shared__ Row row;
+  __shared__ double piece[2][kWarps];  // [residual, target][warp]: sums over the warp's piece
+  __shared__ double totals[2];         // this CTA's
+  __shared__ int pick;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int ranks = (int)cluster.num_blocks();
+  const int seq = blockIdx.x / ranks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0) {  // how many drafts stand (every CTA of the cluster finds the same)
+    Row r;
+    r.begin = __ldg(p.cu + seq);
+    const int end = __ldg(p.cu + seq + 1);
+    r.k = end - r.begin;
+    r.n = 0;
+    r.rejected = -1;
+    if (r.begin < 0 || r.k < 0 || r.k > p.max_drafts || end > p.total) {
+      if (rank == 0 && lane == 0) set_device_error(p.err, B2P_DEV_LENGTH);
+      r.k = -1;
+    }
+    for (int base = 0; base < r.k; base += 32) {
+      const int j = base + lane;
+      bool ok = false;
+      int64_t x = -1;
+      if (j < r.k) {
+        x = p.tokens[r.begin + j];
+        if (x < 0 || x >= p.vocab) {
+          if (rank == 0) set_device_error(p.err, B2P_DEV_TOKEN_RANGE);
+          x = -1;
+        } else {
+          const T* prow = reinterpret_cast<const T*>(p.target) + ((int64_t)r.begin + seq + j) * p.t_row;
+          const T* qrow = reinterpret_cast<const T*>(p.draft) + (int64_t)(r.begin + j) * p.d_row;
+          const double qx = p.draft != nullptr ? (double)to_f32<T>(qrow[x]) : 1.0;
+          ok = (double)p.accept[r.begin + j] * qx < (double)to_f32<T>(prow[x]);
+        }
+      }
+      const unsigned stop = __ballot_sync(0xffffffffu, j < r.k && !ok);
+      if (stop) {
+        const int first = __ffs(stop) - 1;
+        r.n = base + first;
+        r.rejected = __shfl_sync(0xffffffffu, x, first);
+        break;
+      }
+      r.n = min(base + 32, r.k);
+    }
+    if (lane == 0) row = r;
+    if (rank == 0) {
+      int64_t* out = p.out + (int64_t)seq * p.out_row;
+      for (int j = lane; j <= p.max_drafts; j += 32)
+        if (j != r.n || r.k < 0) out[j] = j < r.n ? p.tokens[r.begin + j] : -1;
+      if (lane == 0) p.accepted[seq] = r.n;
+    }
+  }
+  if (threadIdx.x == 0) pick = p.vocab;
+  __syncthreads();
+  if (row.k < 0) return;  // the whole cluster returns
+
+  const bool rejected = row.n < row.k;
+  const T* prow = reinterpret_cast<const T*>(p.target) + ((int64_t)row.begin + seq + row.n) * p.t_row;
+  const T* qrow = rejected && p.draft != nullptr
+                      ? reinterpret_cast<const T*>(p.draft) + (int64_t)(row.begin + row.n) * p.d_row
+                      : nullptr;
+  const int64_t drop = rejected && p.draft == nullptr ? row.rejected : -1;
+  // the vocabulary in ranks * kWarps pieces, in index order
+  const int len = (p.vocab + ranks * kWarps - 1) / (ranks * kWarps);
+  const int v0 = min(p.vocab, (rank * kWarps + warp) * len), v1 = min(p.vocab, v0 + len);
+  double r = 0.0, t = 0.0;
+#pragma unroll 4
+  for (int v = v0 + lane; v < v1; v += 32) {
+    r += residual<T>(prow, qrow, drop, v);
+    t += positive((double)to_f32<T>(prow[v]));
+  }
+  r = warp_sum(r);
+  t = warp_sum(t);
+  if (lane == 0) {
+    piece[0][warp] = r;
+    piece[1][warp] = t;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    double s = 0.0;
+    for (int w = 0; w < kWarps; ++w) s += piece[threadIdx.x][w];
+    totals[threadIdx.x] = s;
+  }
+  cluster.sync();
+  double all[2] = {0.0, 0.0}, before[2] = {0.0, 0.0};
+  double part[2][kCluster];
+  for (int c = 0; c < kCluster; ++c) {
+    for (int k = 0; k < 2; ++k) {
+      part[k][c] = c < ranks ? *cluster.map_shared_rank(&totals[k], c) : 0.0;
+      if (c == rank) before[k] = all[k];
+      all[k] += part[k][c];
+    }
+  }
+  cluster.sync();  // nobody leaves while its totals may still be read
+  // nothing left over (p <= q everywhere): the target row itself
+  const int use = all[0] > 0.0 ? 0 : 1;
+  const double goal = (double)p.sample[seq] * all[use];
+  // the CTA that holds the crossing; where rounding or a draw outside [0, 1) leaves none, the
+  // last one with anything in it
+  int owner = -1, last = -1;
+  double run = 0.0;
+  for (int c = 0; c < ranks; ++c) {
+    run += part[use][c];
+    if (part[use][c] > 0.0) {
+      last = c;
+      if (owner < 0 && run > goal) owner = c;
+    }
+  }
+  if (owner < 0) owner = last;
+  if (owner < 0) {  // a row without a positive entry
+    if (rank == 0 && threadIdx.x == 0) p.out[(int64_t)seq * p.out_row + row.n] = 0;
+    return;
+  }
+  if (owner != rank) return;
+  // the same inside the CTA, over its warps' pieces
+  int ow = -1, lw = -1;
+  double base = before[use], start = base;
+  for (int w = 0; w < kWarps; ++w) {
+    const double next = base + piece[use][w];
+    if (piece[use][w] > 0.0) {
+      lw = w;
+      if (ow < 0) start = base;
+      if (ow < 0 && next > goal) ow = w;
+    }
+    base = next;
+  }
+  const bool crossing = ow >= 0;
+  if (!crossing) ow = lw;
+  // the piece again, a contiguous run per thread
+  const int w0 = min(p.vocab, (rank * kWarps + ow) * len), w1 = min(p.vocab, w0 + len);
+  const int per = (len + kThreads - 1) / kThreads;
+  const int a = min(w1, w0 + (int)threadIdx.x * per), b = min(w1, a + per);
+  const T* qr = use == 0 ? qrow : nullptr;
+  const int64_t dr = use == 0 ? drop : -1;
+  double mine = 0.0;
+  for (int v = a; v < b; ++v) mine += residual<T>(prow, qr, dr, v);
+  double incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  __shared__ double scan[kWarps];
+  __shared__ int tail;
+  if (threadIdx.x == 0) tail = -1;
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  double at = start;
+  for (int w = 0; w < warp; ++w) at += scan[w];
+  at += incl - mine;
+  for (int v = a; v < b; ++v) {
+    const double x = residual<T>(prow, qr, dr, v);
+    at += x;
+    if (x > 0.0) {
+      atomicMax(&tail, v);
+      if (crossing && at > goal) {
+        atomicMin(&pick, v);
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    p.out[(int64_t)seq * p.out_row + row.n] = pick < p.vocab ? pick : tail;
+}
+
+// Greedy form: the target rows are given by their arg-max ids; a draft stands while it equals
+// the id of its row, and the id of the first row that differs (or of the last one) follows.
+__global__ void __launch_bounds__(128) verify_drafts_greedy(const int64_t* ids, const int64_t* tokens,
+                                                            const int32_t* cu, int64_t total,
+                                                            int num_seqs, int max_drafts, int64_t* out,
+                                                            int64_t out_row, int32_t* accepted,
+                                                            int32_t* err) {
+  const int seq = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (seq >= num_seqs) return;
+  const int begin = __ldg(cu + seq), end = __ldg(cu + seq + 1);
+  int k = end - begin, n = 0;
+  if (begin < 0 || k < 0 || k > max_drafts || end > total) {
+    if (lane == 0) set_device_error(err, B2P_DEV_LENGTH);
+    k = -1;
+  }
+  for (int base = 0; base < k; base += 32) {
+    const int j = base + lane;
+    const bool ok = j < k && tokens[begin + j] == ids[begin + seq + j];
+    const unsigned stop = __ballot_sync(0xffffffffu, j < k && !ok);
+    if (stop) {
+      n = base + __ffs(stop) - 1;
+      break;
+    }
+    n = min(base + 32, k);
+  }
+  for (int j = lane; j <= max_drafts; j += 32)
+    out[(int64_t)seq * out_row + j] =
+        k < 0 ? -1 : j < n ? tokens[begin + j] : j == n ? ids[begin + seq + n] : -1;
+  if (lane == 0) accepted[seq] = n;
+}
+
+}  // namespace
+
+extern "C" int b2p_verify_drafts(const void* target_probs, int64_t target_row_stride,
+                                 const void* draft_probs, int64_t draft_row_stride,
+                                 const int64_t* draft_tokens, const int32_t* cu_drafts,
+                                 const float* accept_draws, const float* sample_draws,
+                                 int num_seqs, int64_t total_drafts, int max_drafts, int vocab,
+                                 int dtype, int64_t* out_tokens, int64_t out_row_stride,
+                                 int32_t* out_accepted, int32_t* err_flag, void* stream) {
+  if (num_seqs < 0 || total_drafts < 0 || max_drafts < 0 || vocab <= 0 ||
+      dtype < B2P_BF16 || dtype > B2P_F32)
+    return B2P_EINVAL;
+  if (num_seqs > (1 << 27) || total_drafts > 0x7fffffffLL || vocab > (1 << 30))
+    return B2P_EUNSUPPORTED;
+  if (num_seqs == 0) return B2P_OK;
+  if (!target_probs || !cu_drafts || !sample_draws || !out_tokens || !out_accepted ||
+      (total_drafts > 0 && (!draft_tokens || !accept_draws)) || out_row_stride < max_drafts + 1)
+    return B2P_EINVAL;
+  VerifyParams p;
+  p.target = static_cast<const uint8_t*>(target_probs);
+  p.t_row = target_row_stride;
+  p.draft = static_cast<const uint8_t*>(draft_probs);
+  p.d_row = draft_row_stride;
+  p.tokens = draft_tokens;
+  p.cu = cu_drafts;
+  p.accept = accept_draws;
+  p.sample = sample_draws;
+  p.total = total_drafts;
+  p.num_seqs = num_seqs;
+  p.max_drafts = max_drafts;
+  p.vocab = vocab;
+  p.out = out_tokens;
+  p.out_row = out_row_stride;
+  p.accepted = out_accepted;
+  p.err = err_flag;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)num_seqs * kCluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const void* fn = dtype == B2P_BF16  ? reinterpret_cast<const void*>(&verify_drafts<__nv_bfloat16>)
+                   : dtype == B2P_F16 ? reinterpret_cast<const void*>(&verify_drafts<__half>)
+                                      : reinterpret_cast<const void*>(&verify_drafts<float>);
+  void* args[] = {&p};
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
+  if (e != cudaSuccess) return b2p_host::record_error(e);
+  return b2p_host::check_launch();
+}
+
+extern "C" int b2p_verify_drafts_greedy(const int64_t* target_ids, const int64_t* draft_tokens,
+                                        const int32_t* cu_drafts, int num_seqs,
+                                        int64_t total_drafts, int max_drafts, int64_t* out_tokens,
+                                        int64_t out_row_stride, int32_t* out_accepted,
+                                        int32_t* err_flag, void* stream) {
+  if (num_seqs < 0 || total_drafts < 0 || max_drafts < 0) return B2P_EINVAL;
+  if (num_seqs == 0) return B2P_OK;
+  if (!target_ids || !cu_drafts || !out_tokens || !out_accepted ||
+      (total_drafts > 0 && !draft_tokens) || out_row_stride < max_drafts + 1)
+    return B2P_EINVAL;
+  verify_drafts_greedy<<<(unsigned)((num_seqs + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(
+      target_ids, draft_tokens, cu_drafts, total_drafts, num_seqs, max_drafts, out_tokens,
+      out_row_stride, out_accepted, err_flag);
+  return b2p_host::check_launch();
+}

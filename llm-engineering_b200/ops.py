@@ -376,3 +376,415 @@ def lm_head_argmax(
     if out_max is not None and mx is not out_max:
         out_max[:rows].copy_(mx[:rows])
     return ids[:rows]
+
+
+# ---------------------------------------------------------------------- 8-bit cache, K7 - K9
+FP8_DTYPE = torch.float8_e4m3fn
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """Launch on ``device``'s current stream, whichever device is current."""
+    fn = getattr(_lib.load(), name)
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream(device))
+    _lib.check(rc, name)
+
+
+def _on(device: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            _require_cuda(name, t)
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+
+
+def _err_flag(err_flag: torch.Tensor | None) -> int | None:
+    if err_flag is None:
+        return None
+    _int32("err_flag", err_flag)
+    return err_flag.data_ptr()
+
+
+def _check_fp8_pool(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: torch.Tensor,
+                    value_scales: torch.Tensor, block_size: int) -> None:
+    _check_pool(key_cache, value_cache)
+    if key_cache.dtype != FP8_DTYPE:
+        raise ValueError(f"an 8-bit pool must be {FP8_DTYPE} (got {key_cache.dtype})")
+    layers, slots, hkv, _ = key_cache.shape
+    if block_size <= 0 or slots % block_size:
+        raise ValueError("the pool's slots must be a multiple of block_size")
+    shape = (layers, slots // block_size, hkv)
+    for name, t in (("key_scales", key_scales), ("value_scales", value_scales)):
+        if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 tensor of shape {shape}")
+    _on(key_cache.device, value_cache=value_cache, key_scales=key_scales, value_scales=value_scales)
+
+
+def _check_tables(device: torch.device, num_seqs: int, block_tables: torch.Tensor,
+                  context_lens: torch.Tensor) -> None:
+    _int32("block_tables", block_tables)
+    _int32("context_lens", context_lens)
+    if block_tables.dim() != 2 or block_tables.shape[0] < num_seqs or context_lens.numel() < num_seqs:
+        raise ValueError("block_tables/context_lens must cover every sequence")
+    _on(device, block_tables=block_tables, context_lens=context_lens)
+
+
+def kv_write_fp8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer_index: int,
+    block_tables: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    context_lens: torch.Tensor,
+    max_q_len: int,
+    block_size: int,
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    err_flag: torch.Tensor | None = None,
+) -> None:
+    """K7: append a packed batch's new K/V rows to an 8-bit cache.
+
+    key_cache/value_cache: float8_e4m3fn [layers, slots, kv_heads, head_dim]; key_scales/
+    value_scales: float32 [layers, blocks, kv_heads]; an element stands for code * scale.
+    Sequence i owns rows [cu_seqlens_q[i], cu_seqlens_q[i+1]) of keys/values (bf16, f16 or fp32,
+    any token/head strides) and appends them at positions ``context_lens[i] - q_len ..
+    context_lens[i] - 1`` through its block table. ``max_q_len`` bounds the q_len (a longer
+    sequence is skipped and flagged). A block's scale is the smallest power of two (from 2**-110)
+    that holds its rows; a write that covers the block's first slot starts it anew, any other one
+    rounds the rows before it to the new scale where that grows. A non-finite row makes the
+    scale NaN. Two sequences of one call must not append to the same block.
+    """
+    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
+    dev = key_cache.device
+    n = cu_seqlens_q.numel() - 1
+    _int32("cu_seqlens_q", cu_seqlens_q)
+    _check_tables(dev, n, block_tables, context_lens)
+    _on(dev, cu_seqlens_q=cu_seqlens_q, keys=keys, values=values, err_flag=err_flag)
+    layers, slots, hkv, d = key_cache.shape
+    if keys.shape != values.shape or keys.dim() != 3 or tuple(keys.shape[1:]) != (hkv, d):
+        raise ValueError(f"keys/values must have shape (tokens, {hkv}, {d})")
+    if keys.dtype != values.dtype:
+        raise ValueError("keys/values dtypes differ")
+    kt, kh = _tok_head_strides("keys", keys)
+    vt, vh = _tok_head_strides("values", values)
+    _call("b2p_kv_write_fp8", dev, keys.data_ptr(), kt, kh, values.data_ptr(), vt, vh,
+          key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+          value_scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
+          cu_seqlens_q.data_ptr(), context_lens.data_ptr(), n, keys.shape[0], max_q_len,
+          layer_index, layers, slots, hkv, d, block_size, dtype_code(keys.dtype),
+          _err_flag(err_flag))
+
+
+def kv_read_fp8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer_index: int,
+    slot_mapping: torch.Tensor,
+    block_size: int,
+    dtype: torch.dtype,
+    err_flag: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of the given slots (int32) as values of ``dtype``: (keys, values), each
+    (rows, kv_heads, head_dim). Negative slots give zero rows."""
+    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
+    dev = key_cache.device
+    _int32("slot_mapping", slot_mapping)
+    _on(dev, slot_mapping=slot_mapping, err_flag=err_flag)
+    code = dtype_code(dtype)
+    layers, slots, hkv, d = key_cache.shape
+    n = slot_mapping.numel()
+    keys = torch.empty((n, hkv, d), dtype=dtype, device=dev)
+    values = torch.empty_like(keys)
+    _call("b2p_kv_read_fp8", dev, key_cache.data_ptr(), value_cache.data_ptr(),
+          key_scales.data_ptr(), value_scales.data_ptr(), slot_mapping.data_ptr(), n,
+          keys.data_ptr(), values.data_ptr(), layer_index, layers, slots, hkv, d, block_size, code,
+          _err_flag(err_flag))
+    return keys, values
+
+
+def fp8_workspace_size(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                       max_q_len: int = 1) -> int:
+    return int(_lib.load().b2p_paged_fp8_workspace_size(num_seqs, num_q_heads, num_kv_heads,
+                                                        head_dim, max_q_len))
+
+
+def make_fp8_workspace(max_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                       device: torch.device, max_q_len: int = 1) -> torch.Tensor:
+    """Zero-filled scratch of the attention calls over the 8-bit cache: for up to ``max_seqs``
+    sequences of up to ``max_q_len`` rows, reusable across layers and steps on one stream."""
+    n = fp8_workspace_size(max_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len)
+    return torch.zeros(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def _check_fp8_query(q: torch.Tensor, key_cache: torch.Tensor, out: torch.Tensor | None):
+    if q.dim() != 3 or q.shape[2] != key_cache.shape[3]:
+        raise ValueError("q must be (rows, num_q_heads, head_dim) with the pool's head_dim")
+    code = dtype_code(q.dtype)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and dtype")
+    return code, out
+
+
+def _fp8_workspace(workspace: torch.Tensor | None, n: int, hq: int, hkv: int, d: int,
+                   device: torch.device, max_q_len: int) -> torch.Tensor:
+    if workspace is None:
+        return make_fp8_workspace(n, hq, hkv, d, device, max_q_len)
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor")
+    _on(device, workspace=workspace)
+    return workspace
+
+
+def paged_decode_fp8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer_index: int,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    scale: float,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    err_flag: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """K2 over the 8-bit cache: one query token per sequence attends its paged history.
+
+    q: (num_seqs, num_q_heads, head_dim) in bf16, f16 or fp32; returns out of the same shape.
+    """
+    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
+    dev = key_cache.device
+    code, out = _check_fp8_query(q, key_cache, out)
+    n, hq, d = q.shape
+    layers, slots, hkv, _ = key_cache.shape
+    _check_tables(dev, n, block_tables, context_lens)
+    _on(dev, q=q, out=out, err_flag=err_flag)
+    qt, qh = _tok_head_strides("q", q)
+    ot, oh = _tok_head_strides("out", out)
+    workspace = _fp8_workspace(workspace, n, hq, hkv, d, dev, 1)
+    _call("b2p_paged_decode_fp8", dev, q.data_ptr(), qt, qh, key_cache.data_ptr(),
+          value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
+          layers, slots, block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(),
+          n, hq, hkv, d, block_size, float(scale), out.data_ptr(), ot, oh, workspace.data_ptr(),
+          workspace.numel(), code, _err_flag(err_flag))
+    return out
+
+
+def paged_prefill_fp8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer_index: int,
+    block_tables: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    context_lens: torch.Tensor,
+    max_q_len: int,
+    block_size: int,
+    scale: float,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    err_flag: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """K3 over the 8-bit cache: packed variable-length causal attention over the paged history
+    (the rows of drafted tokens, of prompt slices or of whole prompts).
+
+    q: (rows, num_q_heads, head_dim); sequence i owns rows [cu_seqlens_q[i], cu_seqlens_q[i+1]) and
+    row j of it sits at position ``context_lens[i] - q_len + j``. ``max_q_len`` bounds the q_len
+    (rows of a longer sequence are flagged). Rows of q that no sequence owns are left alone in out.
+    """
+    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
+    dev = key_cache.device
+    code, out = _check_fp8_query(q, key_cache, out)
+    total_q, hq, d = q.shape
+    layers, slots, hkv, _ = key_cache.shape
+    n = cu_seqlens_q.numel() - 1
+    _int32("cu_seqlens_q", cu_seqlens_q)
+    _check_tables(dev, n, block_tables, context_lens)
+    _on(dev, q=q, out=out, cu_seqlens_q=cu_seqlens_q, err_flag=err_flag)
+    qt, qh = _tok_head_strides("q", q)
+    ot, oh = _tok_head_strides("out", out)
+    workspace = _fp8_workspace(workspace, n, hq, hkv, d, dev, max_q_len)
+    _call("b2p_paged_prefill_fp8", dev, q.data_ptr(), qt, qh, key_cache.data_ptr(),
+          value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
+          layers, slots, block_tables.data_ptr(), block_tables.stride(0), cu_seqlens_q.data_ptr(),
+          context_lens.data_ptr(), n, total_q, max_q_len, hq, hkv, d, block_size, float(scale),
+          out.data_ptr(), ot, oh, workspace.data_ptr(), workspace.numel(), code,
+          _err_flag(err_flag))
+    return out
+
+
+def _drafts_out(n: int, max_drafts: int, device: torch.device):
+    return (torch.empty((n, max_drafts + 1), dtype=torch.int64, device=device),
+            torch.empty(n, dtype=torch.int32, device=device))
+
+
+def _check_drafts(device: torch.device, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor,
+                  max_drafts: int) -> int:
+    _int32("cu_drafts", cu_drafts)
+    if draft_tokens.dim() != 1 or draft_tokens.dtype != torch.int64 or not draft_tokens.is_contiguous():
+        raise ValueError("draft_tokens must be a contiguous int64 vector")
+    if max_drafts < 0 or cu_drafts.numel() < 1:
+        raise ValueError("max_drafts must not be negative and cu_drafts needs an entry")
+    _on(device, draft_tokens=draft_tokens, cu_drafts=cu_drafts)
+    return cu_drafts.numel() - 1
+
+
+def verify_drafts(
+    target_probs: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    cu_drafts: torch.Tensor,
+    accept_draws: torch.Tensor,
+    sample_draws: torch.Tensor,
+    max_drafts: int,
+    draft_probs: torch.Tensor | None = None,
+    err_flag: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """K8: verify drafted tokens against the target model's probabilities.
+
+    Sequence i drafted ``draft_tokens[cu_drafts[i]:cu_drafts[i+1]]`` (int64; cu_drafts int32) and
+    owns the rows ``cu_drafts[i] + i .. cu_drafts[i+1] + i`` of target_probs (one more than it
+    drafted; bf16, f16 or fp32, rows contiguous). draft_probs has one row per draft, or is None
+    when every draft is certain (prompt lookup, greedy drafts). Draft j stands while
+    ``accept_draws[j] * q_j(x_j) < p_j(x_j)``; one more token is drawn with ``sample_draws[i]``
+    from max(p - q, 0) of the first rejected row, or from p of the last row. Draws are fp32 in
+    [0, 1). Returns (tokens, accepted): int64 (num_seqs, max_drafts + 1), the standing drafts, then
+    the drawn token, then -1; and int32 (num_seqs,), how many drafts stand.
+    """
+    _require_cuda("target_probs", target_probs)
+    dev = target_probs.device
+    n = _check_drafts(dev, draft_tokens, cu_drafts, max_drafts)
+    total = draft_tokens.numel()
+    code = dtype_code(target_probs.dtype)
+    if target_probs.dim() != 2 or target_probs.shape[0] != total + n or target_probs.stride(1) != 1:
+        raise ValueError(f"target_probs must be ({total + n}, vocab) with contiguous rows")
+    if draft_probs is not None and (
+            draft_probs.dim() != 2 or tuple(draft_probs.shape) != (total, target_probs.shape[1])
+            or draft_probs.dtype != target_probs.dtype or draft_probs.stride(1) != 1):
+        raise ValueError("draft_probs must be (drafts, vocab) in target_probs' dtype with "
+                         "contiguous rows")
+    for name, t, want in (("accept_draws", accept_draws, total), ("sample_draws", sample_draws, n)):
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != want:
+            raise ValueError(f"{name} must be a contiguous float32 tensor of {want} entries")
+    _on(dev, draft_probs=draft_probs, accept_draws=accept_draws, sample_draws=sample_draws,
+        err_flag=err_flag)
+    tokens, accepted = _drafts_out(n, max_drafts, dev)
+    with_q = draft_probs is not None and total > 0
+    _call("b2p_verify_drafts", dev, target_probs.data_ptr(), target_probs.stride(0),
+          draft_probs.data_ptr() if with_q else None, draft_probs.stride(0) if with_q else 0,
+          draft_tokens.data_ptr(), cu_drafts.data_ptr(), accept_draws.data_ptr(),
+          sample_draws.data_ptr(), n, total, max_drafts, target_probs.shape[1], code,
+          tokens.data_ptr(), tokens.stride(0), accepted.data_ptr(), _err_flag(err_flag))
+    return tokens, accepted
+
+
+def verify_drafts_greedy(
+    target_ids: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    cu_drafts: torch.Tensor,
+    max_drafts: int,
+    err_flag: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The greedy form of ``verify_drafts``: target_ids (int64, drafts + num_seqs) holds the
+    arg-max of each target row (what ``lm_head_argmax`` gives); drafts stand while they equal it."""
+    _require_cuda("target_ids", target_ids)
+    dev = target_ids.device
+    n = _check_drafts(dev, draft_tokens, cu_drafts, max_drafts)
+    total = draft_tokens.numel()
+    if target_ids.dtype != torch.int64 or not target_ids.is_contiguous() or \
+            target_ids.numel() != total + n:
+        raise ValueError(f"target_ids must be a contiguous int64 tensor of {total + n} entries")
+    _on(dev, err_flag=err_flag)
+    tokens, accepted = _drafts_out(n, max_drafts, dev)
+    _call("b2p_verify_drafts_greedy", dev, target_ids.data_ptr(), draft_tokens.data_ptr(),
+          cu_drafts.data_ptr(), n, total, max_drafts, tokens.data_ptr(), tokens.stride(0),
+          accepted.data_ptr(), _err_flag(err_flag))
+    return tokens, accepted
+
+
+def _check_pages(key_cache: torch.Tensor, value_cache: torch.Tensor, block_size: int,
+                 key_scales: torch.Tensor | None, value_scales: torch.Tensor | None) -> None:
+    if key_cache.dtype == FP8_DTYPE:
+        if key_scales is None or value_scales is None:
+            raise ValueError("an 8-bit pool needs its key_scales and value_scales")
+        _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
+        return
+    _check_pool(key_cache, value_cache)
+    dtype_code(key_cache.dtype)
+    if key_scales is not None or value_scales is not None:
+        raise ValueError("only an 8-bit pool has scales")
+    if block_size <= 0 or key_cache.shape[1] % block_size:
+        raise ValueError("the pool's slots must be a multiple of block_size")
+    _on(key_cache.device, value_cache=value_cache)
+
+
+def copy_blocks(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    src_blocks: torch.Tensor,
+    dst_blocks: torch.Tensor,
+    block_size: int,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
+    err_flag: torch.Tensor | None = None,
+) -> None:
+    """K9: copy block src_blocks[i] to block dst_blocks[i] in every layer of K and V (and of the
+    scales of an 8-bit pool). int32 CUDA vectors; a pair with a negative id is skipped. Targets
+    must be distinct, and none of them a source of the same call."""
+    _check_pages(key_cache, value_cache, block_size, key_scales, value_scales)
+    _int32("src_blocks", src_blocks)
+    _int32("dst_blocks", dst_blocks)
+    if src_blocks.numel() != dst_blocks.numel():
+        raise ValueError("src_blocks and dst_blocks must have one entry per pair")
+    dev = key_cache.device
+    _on(dev, src_blocks=src_blocks, dst_blocks=dst_blocks, err_flag=err_flag)
+    layers, slots, hkv, d = key_cache.shape
+    _call("b2p_copy_blocks", dev, key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scales),
+          _ptr(value_scales), src_blocks.data_ptr(), dst_blocks.data_ptr(), src_blocks.numel(),
+          layers, slots, hkv, d, key_cache.element_size(), block_size, _err_flag(err_flag))
+
+
+def compact_blocks(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
+    err_flag: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """K9: move the live blocks (those in the first ceil(context / block_size) entries of each
+    row of block_tables) into the first blocks of the pool, in every layer, and rewrite
+    block_tables in place. Returns (new_ids, num_live): int32 (num_blocks,), the new id of each
+    live block and -1 for the others, and int32 (1,). Live blocks already in place stay; the
+    j-th of the others, in ascending order, goes to the j-th free block. A block that no row names
+    counts as free: pass every table that is in use."""
+    _check_pages(key_cache, value_cache, block_size, key_scales, value_scales)
+    dev = key_cache.device
+    n = context_lens.numel()
+    _check_tables(dev, n, block_tables, context_lens)
+    _on(dev, err_flag=err_flag)
+    layers, slots, hkv, d = key_cache.shape
+    blocks = slots // block_size
+    size = int(_lib.load().b2p_compact_blocks_workspace_size(blocks))
+    workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+    new_ids = torch.empty(blocks, dtype=torch.int32, device=dev)
+    num_live = torch.empty(1, dtype=torch.int32, device=dev)
+    _call("b2p_compact_blocks", dev, key_cache.data_ptr(), value_cache.data_ptr(),
+          _ptr(key_scales), _ptr(value_scales), block_tables.data_ptr(), block_tables.stride(0),
+          block_tables.shape[1], context_lens.data_ptr(), n, layers, slots, hkv, d,
+          key_cache.element_size(), block_size, new_ids.data_ptr(), num_live.data_ptr(),
+          workspace.data_ptr(), size, _err_flag(err_flag))
+    return new_ids, num_live
