@@ -170,6 +170,29 @@ int pool_tensor_map(CUtensorMap* out, const void* base, int64_t num_layers, int6
                              head_dim / (128 / elem_bytes));
 }
 
+int fp8_pool_tensor_map(CUtensorMap* out, const void* base, int64_t num_layers, int64_t num_slots,
+                        int num_kv_heads, int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return B2P_EUNSUPPORTED;
+  MapKey k{};
+  k.base = base;
+  k.rank = 5;
+  k.dims[0] = head_dim;
+  k.dims[1] = 1;
+  k.dims[2] = num_kv_heads;
+  k.dims[3] = num_slots;
+  k.dims[4] = num_layers;
+  k.strides[0] = head_dim;
+  k.strides[1] = head_dim;
+  k.strides[2] = static_cast<uint64_t>(num_kv_heads) * head_dim;
+  k.strides[3] = static_cast<uint64_t>(num_slots) * num_kv_heads * head_dim;
+  k.box[0] = head_dim;
+  k.box[1] = k.box[2] = k.box[4] = 1;
+  k.box[3] = 16;
+  k.dtype = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  k.swizzle = head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  return encode_cached(out, k);
+}
+
 // 4-D map over token-major activations [rows, heads, head_dim] (element strides given)
 // with the box {128-byte line, 1 line, 1 head, box_rows rows}.
 int tensor_map_4d_rows(CUtensorMap* out, const void* base, int64_t rows, int heads, int head_dim,

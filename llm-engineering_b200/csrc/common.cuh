@@ -246,4 +246,9 @@ int pool_tensor_map(CUtensorMap* out, const void* base, int64_t num_layers, int6
 int pool_tensor_map_box(CUtensorMap* out, const void* base, int64_t num_layers, int64_t num_slots,
                         int num_kv_heads, int head_dim, int elem_bytes, int box_chunks);
 
+// 5-D map over an 8-bit pool tensor of head_dim 64 or 128 with the box {one head row, 1, 1 head,
+// 16 slots, 1 layer}, swizzled over the row's 64 or 128 bytes.
+int fp8_pool_tensor_map(CUtensorMap* out, const void* base, int64_t num_layers, int64_t num_slots,
+                        int num_kv_heads, int head_dim);
+
 }  // namespace b2p_host
