@@ -332,8 +332,15 @@ B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, cons
  *   workspace : b2p_paged_fp8_workspace_size() bytes, zero before its first use with these heads
  *               and zeroed again after B2P_DEV_WAIT_TIMEOUT; every completed call leaves it
  *               usable for the next one on the stream. Calls that may overlap need one each.
- *   max_q_len : upper bound of the q_len_i; rows of a longer sequence set B2P_DEV_LENGTH.
+ *   max_q_len : upper bound of the q_len_i; rows of a longer sequence set B2P_DEV_LENGTH or
+ *               are computed all the same.
+ *   scratch   : b2p_paged_prefill_fp8_scratch_size() bytes (0 where the call needs none), any
+ *               contents: many rows run on a 16-bit copy of the histories, made by the call.
+ *               table_width is block_table_stride.
  */
+B2P_API size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t table_width,
+                 int num_q_heads, int num_kv_heads, int head_dim, int block_size, int max_q_len,
+                 int dtype);
 B2P_API size_t b2p_paged_fp8_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads,
                                             int head_dim, int max_q_len);
 B2P_API int b2p_paged_decode_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -351,7 +358,8 @@ B2P_API int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_t q
                  const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
                  int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
                  int block_size, float scale, void* out, int64_t out_tok_stride,
-                 int64_t out_head_stride, void* workspace, size_t workspace_size, int dtype,
+                 int64_t out_head_stride, void* workspace, size_t workspace_size, void* scratch,
+                 size_t scratch_size, int dtype,
                  int32_t* err_flag, void* stream);
 
 /*

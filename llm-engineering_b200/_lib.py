@@ -49,6 +49,7 @@ EXPORTED_SYMBOLS = (
     "b2p_kv_read_fp8",
     "b2p_paged_fp8_workspace_size",
     "b2p_paged_decode_fp8",
+    "b2p_paged_prefill_fp8_scratch_size",
     "b2p_paged_prefill_fp8",
     "b2p_verify_drafts",
     "b2p_verify_drafts_greedy",
@@ -122,10 +123,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _i32, _i32, _i32, _i32,
          _i32, _f32, _p, _i64, _i64, _p, _sz, _i32, _p, _p],
     ),
+    "b2p_paged_prefill_fp8_scratch_size": (
+        _sz, [_i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32],
+    ),
     "b2p_paged_prefill_fp8": (
         _i32,
         [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _i32, _i64, _i32,
-         _i32, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _sz, _i32, _p, _p],
+         _i32, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _sz, _p, _sz, _i32, _p, _p],
     ),
     "b2p_verify_drafts": (
         _i32,

@@ -602,7 +602,9 @@ def paged_prefill_fp8(
 
     q: (rows, num_q_heads, head_dim); sequence i owns rows [cu_seqlens_q[i], cu_seqlens_q[i+1]) and
     row j of it sits at position ``context_lens[i] - q_len + j``. ``max_q_len`` bounds the q_len
-    (rows of a longer sequence are flagged). Rows of q that no sequence owns are left alone in out.
+    (rows of a longer sequence are flagged, or computed all the same). Rows of q that no sequence
+    owns are left alone in out. Calls of many rows widen the histories into a 16-bit copy of
+    ``num_seqs * block_tables.shape[1]`` blocks of one layer, allocated for the call.
     """
     _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
     dev = key_cache.device
@@ -616,12 +618,15 @@ def paged_prefill_fp8(
     qt, qh = _tok_head_strides("q", q)
     ot, oh = _tok_head_strides("out", out)
     workspace = _fp8_workspace(workspace, n, hq, hkv, d, dev, max_q_len)
+    size = int(_lib.load().b2p_paged_prefill_fp8_scratch_size(
+        n, block_tables.stride(0), hq, hkv, d, block_size, max_q_len, code))
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _call("b2p_paged_prefill_fp8", dev, q.data_ptr(), qt, qh, key_cache.data_ptr(),
           value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
           layers, slots, block_tables.data_ptr(), block_tables.stride(0), cu_seqlens_q.data_ptr(),
           context_lens.data_ptr(), n, total_q, max_q_len, hq, hkv, d, block_size, float(scale),
-          out.data_ptr(), ot, oh, workspace.data_ptr(), workspace.numel(), code,
-          _err_flag(err_flag))
+          out.data_ptr(), ot, oh, workspace.data_ptr(), workspace.numel(), _ptr(scratch), size,
+          code, _err_flag(err_flag))
     return out
 
 

@@ -49,13 +49,18 @@ def test_attention_refusals():
 
     def prefill(n=1, rows=2, max_q=2, hq=4, hkv=2, d=64, q=FAKE):
         return c.b2p_paged_prefill_fp8(q, 256, 64, FAKE, FAKE, FAKE, FAKE, 0, 1, 64, FAKE, 4, FAKE, FAKE, n, rows,
-                                       max_q, hq, hkv, d, 16, 0.1, FAKE, 256, 64, None, 0, 0, None, None)
+                                       max_q, hq, hkv, d, 16, 0.1, FAKE, 256, 64, None, 0, None, 0, 0, None, None)
 
     assert decode(n=0) == prefill(n=0) == prefill(rows=0) == prefill(max_q=0) == L.B2P_OK
     assert decode(layer=3) == L.B2P_ERANGE
     assert decode(hq=5) == decode(slots=60) == decode(q=None) == decode(dtype=9) == L.B2P_EINVAL
     assert decode(cache=FAKE + 1) == prefill(q=None) == prefill(max_q=-1) == L.B2P_EINVAL
     assert decode(d=60) == decode(d=512) == prefill(d=264) == L.B2P_EUNSUPPORTED
+    # rows that fit no pass of the few-row kernel need the scratch, few rows the workspace
+    assert prefill(rows=200, max_q=200) == decode() == L.B2P_EWORKSPACE
+    assert c.b2p_paged_prefill_fp8_scratch_size(2, 10, 4, 2, 64, 16, 200, 0) >= 2 * 10 * 16 * 2 * 64 * 4
+    assert c.b2p_paged_prefill_fp8_scratch_size(2, 10, 4, 2, 64, 16, 5, 0) == 0
+    assert c.b2p_paged_prefill_fp8_scratch_size(2, 10, 4, 2, 64, 16, 200, 2) == 0
     assert c.b2p_paged_fp8_workspace_size(0, 4, 2, 64, 1) == 0
     assert c.b2p_paged_fp8_workspace_size(4, 12, 2, 128, 1) > 0
 
