@@ -25,8 +25,13 @@
 //    scores, so the weights that matter keep their 11 bits whatever the spread of the scales.
 //    References only move when a score passes them by 2^8 (one warp vote per tile instead of
 //    shuffles and a rescale of O).
-//  * Sequences cut by range boundaries leave partial records (O scaled into [-1, 1] in f16,
-//    then m_x, the sum and the scale in fp32); the last warp to count in merges them.
+//  * Sequences cut by range boundaries leave partial records (O scaled into [-1, 1], then m_x, the
+//    sum and the scale in fp32) in shared memory. When a CTA's warps are through, they merge
+//    their records together, a 16-dim chunk per warp: sequences that lie inside the CTA's range
+//    are finished there, the (at most two) others leave one record per CTA in the workspace, and
+//    the last CTA to count in merges those. With every warp's records in the workspace and one
+//    merging warp per sequence, 8 sequences of 4000 tokens took 48 us, most of it one warp
+//    reading 74 records.
 #include <mutex>
 #include <type_traits>
 
@@ -54,12 +59,14 @@ struct Fp8Params {
   int64_t num_rows;
   int num_seqs, max_q_len;
   int groups_per_seq;  // column groups (virtual sequences) per sequence
-  int group, layer, block_size, hkv;
+  int group, group_inv;  // G and ceil(2^16 / G)
+  int layer, block_size, hkv;
+  int most_keys;         // what a row of the block table reaches
   int64_t num_blocks;
   const float* k_scales;  // layer bases [num_blocks, hkv]
   const float* v_scales;
   float scale_log2;
-  float* partials;    // [hkv][units][2][record]
+  float* joined;      // [hkv][CTAs][2][record]: the CTAs' open sequences
   int32_t* counters;  // [hkv][virtual sequences], zero between launches
   int32_t* err;
 };
@@ -69,21 +76,26 @@ struct Virtual {
   int seq, row0, qlen, ctx, col0, cols, keys;
 };
 
+// Row of a column: col / G, exact for the columns that occur (col * G < 2^16).
+__device__ __forceinline__ int row_of(const Fp8Params& p, int col) {
+  return (int)((unsigned)(col * p.group_inv) >> 16);
+}
+
 template <int NC>
 __device__ __forceinline__ Virtual virtual_of(const Fp8Params& p, int v) {
   Virtual t;
   if (p.cu == nullptr) {
     t.seq = t.row0 = v;
     t.qlen = 1;
-    t.ctx = t.keys = max(0, __ldg(p.ctx + v));
+    t.ctx = t.keys = min(max(0, __ldg(p.ctx + v)), p.most_keys);
     t.col0 = 0;
     t.cols = p.group;
     return t;
   }
-  t.seq = v / p.groups_per_seq;
+  t.seq = p.groups_per_seq == 1 ? v : v / p.groups_per_seq;
   t.row0 = __ldg(p.cu + t.seq);
   const int end = __ldg(p.cu + t.seq + 1);
-  t.ctx = __ldg(p.ctx + t.seq);
+  t.ctx = min(__ldg(p.ctx + t.seq), p.most_keys);
   t.qlen = end - t.row0;
   t.col0 = (v - t.seq * p.groups_per_seq) * NC;
   if (t.qlen <= 0 || t.qlen > p.max_q_len || t.row0 < 0 || end > p.num_rows) t.qlen = 0;
@@ -92,7 +104,7 @@ __device__ __forceinline__ Virtual virtual_of(const Fp8Params& p, int v) {
     t.cols = t.keys = 0;
     return t;
   }
-  const int last = (t.col0 + t.cols - 1) / p.group;  // the group's last row sees the most
+  const int last = row_of(p, t.col0 + t.cols - 1);  // the group's last row sees the most
   t.keys = max(0, t.ctx - t.qlen + last + 1);
   return t;
 }
@@ -102,53 +114,135 @@ __device__ __forceinline__ int tiles_of(const Fp8Params& p, int v, int nv) {
   return v < nv ? (virtual_of<NC>(p, v).keys + kTile - 1) / kTile : 0;
 }
 
-template <int D, int NT>
+// A partial result: O^T / (l s) in MMA fragment order, then per column m_x, the sum l and the
+// scale s = max_d |O / l|. For bf16 output O is kept in f16 (2^-11 of the column's largest
+// value, against an output step of 2^-8). For f16 output it is kept in fp32 (in f16 it would
+// round once more as coarsely as the output), but with four column tiles, whose fp32 records
+// would not fit in shared memory. CTAs' records are fp32.
+template <int D, int NT, bool kWide>
 struct Fp8Record {
-  static constexpr int kOBytes = (D / 16) * NT * 32 * 8;
+  static constexpr int kOBytes = (D / 16) * NT * 32 * (kWide ? 16 : 8);
   static constexpr int kM = kOBytes / 4;  // float index of the references
   static constexpr int kL = kM + NT * 8;  // ... of the sums
   static constexpr int kS = kL + NT * 8;  // ... of the scales
   static constexpr int kFloats = kS + NT * 8;
+
+  __device__ static void put(float* rec, int item, int lane, float a, float b, float c, float d) {
+    if constexpr (kWide)
+      reinterpret_cast<float4*>(rec)[item * 32 + lane] = make_float4(a, b, c, d);
+    else
+      reinterpret_cast<uint2*>(rec)[item * 32 + lane] = make_uint2(pack2<__half>(a, b), pack2<__half>(c, d));
+  }
+  template <bool kGlobal>  // another CTA's record (L2), or this CTA's in shared memory
+  __device__ static float4 get(const float* rec, int item, int lane) {
+    if constexpr (kWide) {
+      const float4* at = reinterpret_cast<const float4*>(rec) + item * 32 + lane;
+      return kGlobal ? __ldcg(at) : *at;
+    } else {
+      const uint2* at = reinterpret_cast<const uint2*>(rec) + item * 32 + lane;
+      const uint2 v = kGlobal ? __ldcg(at) : *at;
+      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+      const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+      return make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+  }
+  template <bool kGlobal>  // the two columns c, c + 1 of field `at`
+  __device__ static float2 pair(const float* rec, int at, int c) {
+    const float2* x = reinterpret_cast<const float2*>(rec + at + c);
+    return kGlobal ? __ldcg(x) : *x;
+  }
 };
 
+// One fragment (item = chunk * NT + nn; a lane's four values of two columns) of records merged.
+template <typename Rec, int NT, bool kGlobal>
+struct Merge {
+  float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+  float o[4] = {0.f, 0.f, 0.f, 0.f};  // O, unnormalised against m
+
+  // kBatch records' loads go out before any of them is used
+  template <int kBatch, typename At>
+  __device__ void run(int count, int item, int lane, const At& at) {
+    const int c = (item % NT) * 8 + 2 * (lane & 3);
+    for (int k0 = 0; k0 < count; k0 += kBatch) {
+      float4 v[kBatch];
+      float2 vm[kBatch], vl[kBatch], vs[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const bool have = k0 + b < count;
+        const float* rec = at(have ? k0 + b : k0);
+        v[b] = Rec::template get<kGlobal>(rec, item, lane);
+        vm[b] = Rec::template pair<kGlobal>(rec, Rec::kM, c);
+        vl[b] = Rec::template pair<kGlobal>(rec, Rec::kL, c);
+        vs[b] = Rec::template pair<kGlobal>(rec, Rec::kS, c);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const float xm[2] = {vm[b].x, vm[b].y}, xl[2] = {vl[b].x, vl[b].y}, xs[2] = {vs[b].x, vs[b].y};
+        const float xo[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+        if (k0 + b >= count) continue;
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const float mn = fmaxf(m[cc], xm[cc]);
+          const float a = fast_exp2(m[cc] - mn), w = fast_exp2(xm[cc] - mn) * xl[cc];
+          m[cc] = mn;
+          l[cc] = l[cc] * a + w;
+          o[cc] = o[cc] * a + xo[cc] * (w * xs[cc]);
+          o[2 + cc] = o[2 + cc] * a + xo[2 + cc] * (w * xs[cc]);
+        }
+      }
+    }
+  }
+};
+
+// The tiles of all virtual sequences in equal ranges: the first `extra` units take base + 1 of
+// them, the others base. (The host bounds the tile count to 31 bits.)
 struct Fp8Range {
-  int64_t begin, end, total, parts, cb0;  // tiles of this unit; first tile of seq0
-  int seq0;
+  int begin, end;            // tiles of this unit
+  int total, parts;          // tiles, units that have any
+  int base, extra;
+  int seq0, cb0;             // virtual sequence of `begin` and its first tile
+  bool odd;                  // some virtual sequence has no tile (nothing to see, or refused)
+
+  __device__ __forceinline__ int start(int c) const { return c * base + min(c, extra); }
+  __device__ __forceinline__ int unit_of(int b) const {
+    const int cut = extra * (base + 1);
+    return b < cut ? b / (base + 1) : extra + (b - cut) / base;
+  }
 };
-
-__device__ __forceinline__ int64_t unit_start(int64_t c, int64_t total, int64_t parts) {
-  return (c * total) / parts;
-}
-
-__device__ __forceinline__ int64_t unit_of(int64_t b, int64_t total, int64_t parts) {
-  return ((b + 1) * parts - 1) / total;
-}
 
 // One warp: all tiles counted, then the virtual sequence that holds unit c's first one. A lane
 // owns kPer consecutive ones of a 32 * kPer chunk and loads them before any arithmetic.
 template <int NC>
-__device__ void find_unit(const Fp8Params& p, int nv, int64_t parts, int64_t c, Fp8Range& r) {
+__device__ void find_unit(const Fp8Params& p, int nv, int units, int c, Fp8Range& r) {
   constexpr int kPer = 8, kChunk = 32 * kPer;
   const int lane = threadIdx.x & 31;
   int nt[kPer];
-  int64_t total = 0;
+  int total = 0;
+  bool odd = false;
   for (int base = 0; base < nv; base += kChunk) {
     int sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) nt[j] = tiles_of<NC>(p, base + lane * kPer + j, nv);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += nt[j];
-    total += __reduce_add_sync(0xffffffffu, (unsigned)sum);
+    for (int j = 0; j < kPer; ++j) {
+      sum += nt[j];
+      odd |= nt[j] == 0 && base + lane * kPer + j < nv;
+    }
+    total += (int)__reduce_add_sync(0xffffffffu, (unsigned)sum);
   }
+  r.odd = __any_sync(0xffffffffu, odd);
   r.total = total;
-  r.parts = parts < total ? parts : total;  // every range holds a tile
+  r.parts = min(units, total);  // every range holds a tile
   r.seq0 = nv;
   r.cb0 = total;
-  r.begin = r.end = 0;
+  r.begin = r.end = r.base = r.extra = 0;
+  if (total == 0) return;
+  r.base = total / r.parts;
+  r.extra = total - r.base * r.parts;
   if (c >= r.parts) return;
-  r.begin = unit_start(c, total, r.parts);
-  r.end = unit_start(c + 1, total, r.parts);
-  int64_t run = 0;
+  r.begin = r.start(c);
+  r.end = r.start(c + 1);
+  int run = 0;
   for (int base = 0; base < nv; base += kChunk) {
     if (nv > kChunk) {  // the registers hold the last chunk only
 #pragma unroll
@@ -166,23 +260,17 @@ __device__ void find_unit(const Fp8Params& p, int nv, int64_t parts, int64_t c, 
     const unsigned hit = __ballot_sync(0xffffffffu, run + incl > r.begin);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      int seq = 0;
-      int64_t cb = run + incl - sum;
-      if (lane == src) {
-        int k = 0;
-        bool found = false;
+      int k = 0, cb = run + incl - sum;
+      bool found = false;
 #pragma unroll
-        for (int j = 0; j < kPer - 1; ++j) {
-          if (!found && cb + nt[j] <= r.begin) {
-            cb += nt[j];
-            k = j + 1;
-          } else {
-            found = true;
-          }
+      for (int j = 0; j < kPer - 1; ++j) {
+        found |= cb + nt[j] > r.begin;
+        if (!found) {
+          cb += nt[j];
+          k = j + 1;
         }
-        seq = base + lane * kPer + k;
       }
-      r.seq0 = __shfl_sync(0xffffffffu, seq, src);
+      r.seq0 = __shfl_sync(0xffffffffu, base + lane * kPer + k, src);
       r.cb0 = __shfl_sync(0xffffffffu, cb, src);
       return;
     }
@@ -199,16 +287,15 @@ struct Slots {
 
 template <int NC>
 struct TileResolver {
-  int win;         // first virtual sequence that can hold the next chunk
-  int64_t win_cb;  // its first tile
-  int64_t begin, n;
+  int win;     // first virtual sequence that can hold the next chunk
+  int win_cb;  // its first tile
+  int begin, n;
 
-  __device__ Slots operator()(const Fp8Params& p, int nv, int64_t chunk0, int lane, int32_t num_slots) {
+  __device__ Slots operator()(const Fp8Params& p, int nv, int chunk0, int lane, int32_t num_slots) {
     const unsigned all = 0xffffffffu;
-    const int64_t g = begin + chunk0 + lane;
+    const int g = begin + chunk0 + lane;
     const bool valid = chunk0 + lane < n;
-    int my = -1;
-    int64_t my_cb = 0;
+    int my = -1, my_cb = 0;
     while (true) {  // windows of 32 virtual sequences
       const int nt = tiles_of<NC>(p, win + lane, nv);
       int incl = nt;
@@ -217,17 +304,17 @@ struct TileResolver {
         const int y = __shfl_up_sync(all, incl, o);
         if (lane >= o) incl += y;
       }
-      const int64_t end = win_cb + incl;
+      const int end = win_cb + incl;
       int lo = 0, hi = 32;  // smallest j whose end passes g
 #pragma unroll
       for (int step = 0; step < 6; ++step) {
         const int mid = (lo + hi) >> 1;
-        const int64_t e = __shfl_sync(all, end, mid < 32 ? mid : 31);
+        const int e = __shfl_sync(all, end, mid < 32 ? mid : 31);
         if (lo < hi) {
           if (e > g) hi = mid; else lo = mid + 1;
         }
       }
-      const int64_t first = __shfl_sync(all, end - nt, lo < 32 ? lo : 31);
+      const int first = __shfl_sync(all, end - nt, lo < 32 ? lo : 31);
       if (valid && my < 0 && lo < 32) {
         my = win + lo;
         my_cb = first;
@@ -250,18 +337,18 @@ struct TileResolver {
       return s;
     }
     const Virtual v = virtual_of<NC>(p, my);
-    const int tok = (int)(g - my_cb) * kTile;
+    const int tok = (g - my_cb) * kTile;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int t = tok + h * kSub;
       if (t >= v.keys) continue;
-      const int64_t col = t / p.block_size;
-      const int32_t blk = col < p.bt_stride ? __ldg(p.block_tables + (int64_t)v.seq * p.bt_stride + col) : -1;
+      const int col = t / p.block_size;  // < the table's width: keys end at most_keys
+      const int32_t blk = __ldg(p.block_tables + (int64_t)v.seq * p.bt_stride + col);
       if (blk < 0 || blk >= p.num_blocks) {
         set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
       } else {
         s.block[h] = blk;
-        s.slot[h] = blk * p.block_size + t % p.block_size;
+        s.slot[h] = blk * p.block_size + t - col * p.block_size;
       }
     }
     return s;
@@ -270,7 +357,8 @@ struct TileResolver {
 
 // Byte offset of 16-byte chunk `chunk` of token row `tok` in a box of D-byte rows, as the TMA
 // unit swizzles it (128-byte rows: chunk ^ row mod 8; 64-byte rows: chunk ^ row / 2 mod 4): the
-// eight rows of an ldmatrix phase then lie in eight different 16-byte bank groups.
+// eight rows of an ldmatrix phase then lie in eight different 16-byte bank groups. For a fixed
+// row and an even c, the offset of chunk c + dc is that of chunk dc with bits 5.. flipped by c.
 template <int D>
 __device__ __forceinline__ uint32_t box_off(int tok, int chunk) {
   return D == 128 ? (uint32_t)(tok * 128 + ((chunk ^ (tok & 7)) << 4))
@@ -294,7 +382,16 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   constexpr int kStage = 4 * kBox;          // K lo, K hi, V lo, V hi
   constexpr bool kQShared = NT > 2;         // Q fragments in shared memory
   constexpr int kQBytes = kQShared ? kChunks * NT * 32 * 8 : 0;
-  using Rec = Fp8Record<D, NT>;
+  using Rec = Fp8Record<D, NT, std::is_same<T, __half>::value && NT <= 2>;  // a warp's
+  using Joined = Fp8Record<D, NT, true>;                                   // a CTA's
+  struct Cut {  // a segment that a warp left as a record, in shared memory
+    int v, nt;
+    int in_ring;  // the stream's last segment: in the warp's ring, done with by then
+    int cb;       // first tile of v
+  };
+  __shared__ Cut cuts[W][2];
+  __shared__ int num_cuts[W];
+  __shared__ int last_of[2];  // per open group: this CTA was the last to count in
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // Programmatic dependent launch, as in the 16-bit decode kernel: before the wait only
@@ -305,7 +402,12 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   const int head = blockIdx.y;
   uint8_t* ring = smem + (size_t)warp * S * kStage;
   uint2* qsm = reinterpret_cast<uint2*>(smem + (size_t)W * S * kStage + (size_t)warp * kQBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)W * (S * kStage + kQBytes)) + warp * S;
+  uint8_t* firsts = smem + (size_t)W * (S * kStage + kQBytes);  // [W][record]: cuts in mid-stream
+  uint64_t* full = reinterpret_cast<uint64_t*>(firsts + (size_t)W * Rec::kFloats * 4) + warp * S;
+  static_assert(Rec::kFloats * 4 <= S * kStage && Rec::kFloats % 4 == 0, "a ring holds a record");
+  auto record_of = [&](int w, bool in_ring) {
+    return reinterpret_cast<float*>(in_ring ? smem + (size_t)w * S * kStage : firsts + (size_t)w * Rec::kFloats * 4);
+  };
   const int nv = p.num_seqs * p.groups_per_seq;
   const int32_t num_slots = (int32_t)(p.num_blocks * p.block_size);
   const int g8 = lane >> 2, t4 = lane & 3;
@@ -319,7 +421,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       if (v < nv) {
         const Virtual t = virtual_of<NC>(p, v);
         empty = t.cols > 0 && t.keys <= 0;
-        bad = empty || (p.cu != nullptr && t.cols > 0 && t.ctx < t.qlen);
+        bad = empty;
         if (p.cu != nullptr && t.qlen == 0) {  // refused offsets, or simply no rows
           const int n = __ldg(p.cu + t.seq + 1) - t.row0;
           bad |= n > p.max_q_len || n < 0 || t.row0 < 0 || (int64_t)t.row0 + n > p.num_rows;
@@ -342,14 +444,14 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   const bool empties_warp = blockIdx.x == 0 && warp == W - 1;
 
   Fp8Range r;
-  const int64_t unit = (int64_t)blockIdx.x * W + warp;
-  find_unit<NC>(p, nv, (int64_t)gridDim.x * W, unit, r);
-  if (r.begin >= r.end) {
+  const int unit = blockIdx.x * W + warp;
+  find_unit<NC>(p, nv, gridDim.x * W, unit, r);
+  if ((int)blockIdx.x * W >= r.parts) {  // no tile for this CTA
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (empties_warp) write_empties();
     return;
   }
-  const int64_t n = r.end - r.begin;
+  const int n = r.end - r.begin;  // 0 for a warp without tiles
   if (lane == 0) {
     for (int s = 0; s < S; ++s) mbar_init(&full[s], 1);
     fence_mbar_init();
@@ -384,40 +486,36 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   };
   load_scales(cur, ks_cur, vs_cur);
   ks_nxt[0] = ks_nxt[1] = vs_nxt[0] = vs_nxt[1] = 0.f;
-  int64_t issue_base = 0;  // tiles [issue_base, issue_base + 32) are in the issue slots
-  Slots isl = cur;         // slots that the issue side reads (may run a chunk ahead of the scales)
-  int64_t issued = 0, use_base = 0;
+  int issue_base = 0;  // tiles [issue_base, issue_base + 32) are in the issue slots
+  Slots isl = cur;     // slots that the issue side reads (may run a chunk ahead of the scales)
+  int issued = 0, use_base = 0, issue_stage = 0;
   bool aborted = false;
 
-  auto issue = [&](int64_t k) {
-    if (k >= issue_base + 32) {
+  auto issue = [&]() {  // tile `issued` into the next stage
+    if (issued >= issue_base + 32) {
       issue_base += 32;
       isl = nxt;
     }
-    const int32_t s0 = __shfl_sync(0xffffffffu, isl.slot[0], (int)(k - issue_base));
-    const int32_t s1 = __shfl_sync(0xffffffffu, isl.slot[1], (int)(k - issue_base));
+    const int32_t s0 = __shfl_sync(0xffffffffu, isl.slot[0], issued - issue_base);
+    const int32_t s1 = __shfl_sync(0xffffffffu, isl.slot[1], issued - issue_base);
     if (lane == 0) {
-      const int st = (int)(k % S);
-      uint8_t* dst = ring + st * kStage;
-      mbar_arrive_expect_tx(&full[st], kStage);
-      tma_load_5d(dst, &kmap, &full[st], 0, 0, head, s0, p.layer);
-      tma_load_5d(dst + kBox, &kmap, &full[st], 0, 0, head, s1, p.layer);
-      tma_load_5d(dst + 2 * kBox, &vmap, &full[st], 0, 0, head, s0, p.layer);
-      tma_load_5d(dst + 3 * kBox, &vmap, &full[st], 0, 0, head, s1, p.layer);
+      uint8_t* dst = ring + issue_stage * kStage;
+      uint64_t* bar = full + issue_stage;
+      mbar_arrive_expect_tx(bar, kStage);
+      tma_load_5d(dst, &kmap, bar, 0, 0, head, s0, p.layer);
+      tma_load_5d(dst + kBox, &kmap, bar, 0, 0, head, s1, p.layer);
+      tma_load_5d(dst + 2 * kBox, &vmap, bar, 0, 0, head, s0, p.layer);
+      tma_load_5d(dst + 3 * kBox, &vmap, bar, 0, 0, head, s1, p.layer);
     }
-    issued = k + 1;
+    ++issued;
+    issue_stage = issue_stage + 1 == S ? 0 : issue_stage + 1;
   };
-  for (int64_t k = 0; k < S && k < n; ++k) issue(k);
-  if (empties_warp) write_empties();  // while the first tiles are in flight
-  if (n > 32) {
-    nxt = res(p, nv, 32, lane, num_slots);
-    load_scales(nxt, ks_nxt, vs_nxt);
-  }
+#pragma unroll
+  for (int k = 0; k < S; ++k)
+    if (k < n) issue();
+  if (empties_warp && r.odd) write_empties();  // while the first tiles are in flight
 
-  int npend = 0;  // virtual sequences left as partials (at most the unit's first and last)
-  int pend_v[2] = {0, 0};
-  int64_t pend_cb[2] = {0, 0};
-  int pend_nt[2] = {0, 0};
+  int ncut = 0;  // records left (at most the unit's first and last segment)
 
   // Rows of one virtual sequence from O^T fragments: out = O * factor.
   auto write_out = [&](const Virtual& t, float (&o)[kChunks][NT][4], float (&f)[NT][2]) {
@@ -428,8 +526,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         const int c = nn * 8 + 2 * t4 + cc;
         if (c >= t.cols) continue;
         const int col = t.col0 + c;
-        T* orow = reinterpret_cast<T*>(p.out) + (int64_t)(t.row0 + col / p.group) * p.o_tok +
-                  (int64_t)(head * p.group + col % p.group) * p.o_head;
+        T* orow = reinterpret_cast<T*>(p.out) + (int64_t)(t.row0 + row_of(p, col)) * p.o_tok +
+                  (int64_t)(head * p.group + col - row_of(p, col) * p.group) * p.o_head;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
           *reinterpret_cast<uint32_t*>(orow + i * 16 + 2 * g8) =
@@ -439,7 +537,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   };
 
   int v = r.seq0;
-  int64_t cb = r.cb0, gidx = r.begin, k = 0;
+  int cb = r.cb0, gidx = r.begin, k = 0, use_stage = 0;
+  uint32_t phase = 0;
   while (gidx < r.end) {
     const Virtual t = virtual_of<NC>(p, v);
     const int ntl = (t.keys + kTile - 1) / kTile;
@@ -447,9 +546,13 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       ++v;
       continue;
     }
-    const int lb0 = (int)(gidx - cb);
-    const int64_t seg_end = min(r.end, cb + ntl);
-    const int lb1 = (int)(seg_end - cb);
+    const int lb0 = gidx - cb;
+    const int seg_end = min(r.end, cb + ntl);
+    const int lb1 = seg_end - cb;
+    if (lane == 0) {
+      if (p.cu != nullptr && t.ctx < t.qlen) set_device_error(p.err, B2P_DEV_LENGTH);
+      if (__ldg(p.ctx + t.seq) > p.most_keys) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
+    }
 
     // ---- Q fragments: column nn * 8 + g8, dims 16c + 4 t4 .. + 3 (8 bytes per lane and k-step)
     uint2 qf[kQShared ? 1 : kChunks][kQShared ? 1 : NT];
@@ -459,8 +562,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       const int c = nn * 8 + g8;
       const bool ok = c < t.cols;
       const int col = t.col0 + (ok ? c : 0);
-      const T* qrow = reinterpret_cast<const T*>(p.q) + (int64_t)(t.row0 + col / p.group) * p.q_tok +
-                      (int64_t)(head * p.group + col % p.group) * p.q_head + 4 * t4;
+      const T* qrow = reinterpret_cast<const T*>(p.q) + (int64_t)(t.row0 + row_of(p, col)) * p.q_tok +
+                      (int64_t)(head * p.group + col - row_of(p, col) * p.group) * p.q_head + 4 * t4;
       uint2 w[kChunks];
 #pragma unroll
       for (int kk = 0; kk < kChunks; ++kk)
@@ -506,9 +609,9 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc) {
         const int c = nn * 8 + 2 * t4 + cc;
-        lim[nn][cc] = p.cu == nullptr ? t.keys : c < t.cols ? t.ctx - t.qlen + (t.col0 + c) / p.group + 1 : t.keys;
+        lim[nn][cc] = p.cu == nullptr ? t.keys : c < t.cols ? t.ctx - t.qlen + row_of(p, t.col0 + c) + 1 : t.keys;
       }
-    if (p.cu != nullptr) lim_min = t.ctx - t.qlen + t.col0 / p.group + 1;
+    if (p.cu != nullptr) lim_min = t.ctx - t.qlen + row_of(p, t.col0) + 1;
 
     float mx[NT][2], my[NT][2], gy[NT][2], l[NT][2];
     float acc[kChunks][NT][4];
@@ -524,26 +627,29 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       for (int nn = 0; nn < NT; ++nn) acc[i][nn][0] = acc[i][nn][1] = acc[i][nn][2] = acc[i][nn][3] = 0.f;
 
     for (int lb = lb0; lb < lb1; ++lb, ++k) {
-      if (k >= use_base + 32) {  // rotate the scale buffers; the issue side has moved on already
+      if (k == use_base + 32) {  // rotate the scale buffers; the issue side has moved on already
         use_base += 32;
         ks_cur[0] = ks_nxt[0], ks_cur[1] = ks_nxt[1], vs_cur[0] = vs_nxt[0], vs_cur[1] = vs_nxt[1];
-        if (use_base + 32 < n) {
-          nxt = res(p, nv, use_base + 32, lane, num_slots);
-          load_scales(nxt, ks_nxt, vs_nxt);
-        }
       }
-      const int src = (int)(k - use_base);
+      if (k == use_base + 8 && use_base + 32 < n) {  // the next chunk, well before it is issued
+        nxt = res(p, nv, use_base + 32, lane, num_slots);
+        load_scales(nxt, ks_nxt, vs_nxt);
+      }
+      const int src = k - use_base;
       float ks[2], vs[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         ks[h] = __shfl_sync(0xffffffffu, ks_cur[h], src);
         vs[h] = __shfl_sync(0xffffffffu, vs_cur[h], src);
       }
-      const int st = (int)(k % S);
-      if (!aborted && !mbar_wait_bounded(&full[st], (uint32_t)((k / S) & 1), p.err)) aborted = true;
+      if (!aborted && !mbar_wait_bounded(full + use_stage, phase, p.err)) aborted = true;
       aborted = __any_sync(0xffffffffu, aborted);
       if (aborted) continue;  // keep walking so every sequence still gets written
-      uint8_t* stage = ring + st * kStage;
+      uint8_t* stage = ring + use_stage * kStage;
+      if (++use_stage == S) {
+        use_stage = 0;
+        phase ^= 1u;
+      }
       const int tok0 = lb * kTile;
       const int valid = min(kTile, t.ctx - tok0);  // tokens that exist
       if (valid < kTile) {
@@ -566,7 +672,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 #pragma unroll
         for (int nn = 0; nn < NT; ++nn) s[h][nn][0] = s[h][nn][1] = s[h][nn][2] = s[h][nn][3] = 0.f;
       {
-        const int tok = (lane & 7) + ((lane >> 3) & 1) * 8, dc = lane >> 4;
+        const uint32_t mine = base + box_off<D>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
           uint2 b[2][NT];
@@ -578,7 +684,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t a0, a1, a2, a3;
-            ldmatrix_x4(base + h * kBox + box_off<D>(tok, c + dc), a0, a1, a2, a3);
+            ldmatrix_x4((mine + h * kBox) ^ (uint32_t)(c << 4), a0, a1, a2, a3);
 #pragma unroll
             for (int nn = 0; nn < NT; ++nn)
               MmaOp<__half>::run(s[h][nn], cvt_lo(a0), cvt_lo(a1), cvt_hi(a0), cvt_hi(a1), b[0][nn].x, b[0][nn].y);
@@ -665,13 +771,13 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 
       // ---- O^T += V^T P^T: 16 dims per fragment (even ones in rows 0..7, odd ones in 8..15)
       {
-        const int tok = (lane & 7) + ((lane >> 3) & 1) * 8, dc = lane >> 4;
+        const uint32_t mine = base + 2 * kBox + box_off<D>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t a0, a1, a2, a3;
-            ldmatrix_x4_trans(base + (2 + h) * kBox + box_off<D>(tok, c + dc), a0, a1, a2, a3);
+            ldmatrix_x4_trans((mine + h * kBox) ^ (uint32_t)(c << 4), a0, a1, a2, a3);
             a0 = __byte_perm(a0, 0, 0x3120), a1 = __byte_perm(a1, 0, 0x3120);
             a2 = __byte_perm(a2, 0, 0x3120), a3 = __byte_perm(a3, 0, 0x3120);
 #pragma unroll
@@ -687,7 +793,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       // the TMA unit writes the same bytes.
       if (valid < kTile) fence_proxy_async_smem();
       __syncwarp();
-      if (k + S < n) issue(k + S);
+      if (issued < n) issue();
     }
 
     // ---- finish the segment
@@ -707,8 +813,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
           f[nn][cc] = l[nn][cc] > 0.f ? fast_exp2(my[nn][cc] - mx[nn][cc]) / l[nn][cc] : 0.f;
       write_out(t, acc, f);
     } else {
-      const int which = (cb + lb0 == r.begin) ? 0 : 1;  // the unit's first segment or a later one
-      float* rec = p.partials + (((size_t)head * r.parts + unit) * 2 + which) * Rec::kFloats;
+      const bool in_ring = seg_end == r.end;
+      float* rec = record_of(warp, in_ring);
 #pragma unroll
       for (int nn = 0; nn < NT; ++nn) {
         float top[2] = {0.f, 0.f};
@@ -725,9 +831,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         const float f0 = top[0] > 0.f ? 1.f / top[0] : 0.f, f1 = top[1] > 0.f ? 1.f / top[1] : 0.f;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
-          reinterpret_cast<uint2*>(rec)[(i * NT + nn) * 32 + lane] =
-              make_uint2(pack2<__half>(acc[i][nn][0] * f0, acc[i][nn][1] * f1),
-                         pack2<__half>(acc[i][nn][2] * f0, acc[i][nn][3] * f1));
+          Rec::put(rec, i * NT + nn, lane, acc[i][nn][0] * f0, acc[i][nn][1] * f1, acc[i][nn][2] * f0, acc[i][nn][3] * f1);
         if (g8 == 0) {
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
@@ -738,12 +842,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
           }
         }
       }
-      if (npend < 2) {  // counted in after the stream: a fence now would stall its refills
-        pend_v[npend] = v;
-        pend_cb[npend] = cb;
-        pend_nt[npend] = ntl;
-        ++npend;
-      }
+      if (lane == 0 && ncut < 2) cuts[warp][ncut] = Cut{v, ntl, in_ring, cb};
+      ++ncut;
     }
     gidx = seg_end;
     if (lb1 == ntl) {
@@ -752,94 +852,107 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
     }
   }
   // Never leave with TMA writes in flight (only after an abort: every issued tile is waited for).
-  if (lane == 0)
-    for (int64_t kk = k; kk < issued; ++kk) mbar_wait_bounded(&full[kk % S], (uint32_t)((kk / S) & 1), nullptr);
+  if (aborted && lane == 0)
+    for (int st = 0; st < S; ++st) {  // a stage's last load has completed when its phase flips
+      const int loads = (issued + S - 1 - st) / S;
+      if (loads > 0) mbar_wait_bounded(full + st, (uint32_t)((loads - 1) & 1), nullptr);
+    }
 
-  // ---- count this warp's partials in; the last one of a virtual sequence merges them
-  int last_mask = 0;
-  __syncwarp();
-  if (lane == 0 && npend > 0) {
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");  // the warp's records before its counts
-    int prev[2] = {0, 0};
-    for (int j = 0; j < npend; ++j) prev[j] = atomicAdd(p.counters + (size_t)head * nv + pend_v[j], 1);
-    for (int j = 0; j < npend; ++j) {
-      const int64_t uf = unit_of(pend_cb[j], r.total, r.parts);
-      const int64_t ul = unit_of(pend_cb[j] + pend_nt[j] - 1, r.total, r.parts);
-      if (prev[j] == (int)(ul - uf)) {
-        p.counters[(size_t)head * nv + pend_v[j]] = 0;
-        last_mask |= 1 << j;
+  // ---- merge what this CTA's warps left. The cuts, in tile order, fall into groups of one
+  // virtual sequence each; all warps walk the groups together.
+  if (lane == 0) num_cuts[warp] = ncut;
+  __syncthreads();
+  const int cta_unit = blockIdx.x * W;
+  const int cta_begin = r.start(cta_unit), cta_end = r.start(min(cta_unit + W, r.parts));
+  auto write_item = [&](int v, int item, const float (&o)[4], const float (&l)[2]) {
+    const Virtual t = virtual_of<NC>(p, v);
+    const int i = item / NT, nn = item % NT;
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc) {
+      const int c = nn * 8 + 2 * t4 + cc;
+      if (c >= t.cols) continue;
+      const int col = t.col0 + c;
+      const float f = l[cc] > 0.f ? 1.f / l[cc] : 0.f;
+      T* orow = reinterpret_cast<T*>(p.out) + (int64_t)(t.row0 + row_of(p, col)) * p.o_tok +
+                (int64_t)(head * p.group + col - row_of(p, col) * p.group) * p.o_head;
+      *reinterpret_cast<uint32_t*>(orow + i * 16 + 2 * g8) = pack2<T>(o[cc] * f, o[2 + cc] * f);
+    }
+  };
+  constexpr int kItems = kChunks * NT;
+  int open_v[2], open_cb[2], open_c0[2], open_c1[2];  // sequences that CTAs c0 .. c1 share
+  int opens = 0;
+  for (int w = 0, c = 0;;) {
+    while (w < W && c >= num_cuts[w]) ++w, c = 0;
+    if (w == W) break;
+    const Cut g = cuts[w][c];
+    // the group: this cut and the first one of each further warp up to the sequence's end
+    const int u1 = r.unit_of(g.cb + g.nt - 1);
+    const int w1 = min(W - 1, u1 - cta_unit);
+    const bool whole = g.cb >= cta_begin && g.cb + g.nt <= cta_end;
+    float* joined = p.joined + (((size_t)head * gridDim.x + blockIdx.x) * 2 + (g.cb <= cta_begin ? 0 : 1)) * Joined::kFloats;
+    for (int item = warp; item < kItems; item += W) {
+      Merge<Rec, NT, false> mg;
+      mg.template run<2>(w1 - w + 1, item, lane, [&](int k) -> const float* {
+        return record_of(w + k, (k == 0 ? g : cuts[w + k][0]).in_ring);
+      });
+      if (whole) {
+        write_item(g.v, item, mg.o, mg.l);
+        continue;
+      }
+      const float i0 = mg.l[0] > 0.f ? 1.f / mg.l[0] : 0.f, i1 = mg.l[1] > 0.f ? 1.f / mg.l[1] : 0.f;
+      Joined::put(joined, item, lane, mg.o[0] * i0, mg.o[1] * i1, mg.o[2] * i0, mg.o[3] * i1);
+      if (item < NT && g8 == 0) {
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          joined[Joined::kM + item * 8 + 2 * t4 + cc] = mg.m[cc];
+          joined[Joined::kL + item * 8 + 2 * t4 + cc] = mg.l[cc];
+          joined[Joined::kS + item * 8 + 2 * t4 + cc] = 1.f;
+        }
       }
     }
-    if (last_mask) asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    if (!whole && opens < 2) {
+      open_v[opens] = g.v;
+      open_cb[opens] = g.cb;
+      open_c0[opens] = r.unit_of(g.cb) / W;
+      open_c1[opens] = u1 / W;
+      ++opens;
+    }
+    if (w1 == w) {
+      ++c;
+    } else {
+      w = w1;
+      c = 1;
+    }
   }
-  last_mask = __shfl_sync(0xffffffffu, last_mask, 0);
-  for (int j = 0; j < npend; ++j) {
-    if (!((last_mask >> j) & 1)) continue;
-    const int64_t scb = pend_cb[j];
-    const int64_t u0 = unit_of(scb, r.total, r.parts), u1 = unit_of(scb + pend_nt[j] - 1, r.total, r.parts);
-    float M[NT][2], L[NT][2];
-    float O[kChunks][NT][4];
+  if (opens == 0) return;  // the same for the whole CTA
+  __syncthreads();  // the CTA's joined records are written
+  if (threadIdx.x == 0) {
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    int seen[2];
 #pragma unroll
-    for (int nn = 0; nn < NT; ++nn) {
-      M[nn][0] = M[nn][1] = kNoMax;
-      L[nn][0] = L[nn][1] = 0.f;
+    for (int j = 0; j < 2; ++j)  // both in flight together
+      seen[j] = j < opens ? atomicAdd(p.counters + (size_t)head * nv + open_v[j], 1) : -1;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) O[i][nn][0] = O[i][nn][1] = O[i][nn][2] = O[i][nn][3] = 0.f;
+    for (int j = 0; j < 2; ++j) {
+      if (j >= opens) continue;
+      const bool is_last = seen[j] == open_c1[j] - open_c0[j];
+      last_of[j] = is_last;
+      if (is_last) p.counters[(size_t)head * nv + open_v[j]] = 0;  // for the next launch
     }
-    constexpr int kBatch = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // records loaded together (registers)
-    for (int64_t ub = u0; ub <= u1; ub += kBatch) {
-      float mv[kBatch][NT][2], lv[kBatch][NT][2], sv[kBatch][NT][2];
-      uint2 ov[kBatch][kChunks][NT];
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int64_t u = ub + b;
-        const bool have = u <= u1;
-        const int which = (u == u0 && unit_start(u, r.total, r.parts) != scb) ? 1 : 0;
-        const float* pr = p.partials + (((size_t)head * r.parts + (have ? u : u0)) * 2 + which) * Rec::kFloats;
-#pragma unroll
-        for (int nn = 0; nn < NT; ++nn) {
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            mv[b][nn][cc] = have ? __ldcg(pr + Rec::kM + nn * 8 + 2 * t4 + cc) : kNoMax;
-            lv[b][nn][cc] = have ? __ldcg(pr + Rec::kL + nn * 8 + 2 * t4 + cc) : 0.f;
-            sv[b][nn][cc] = have ? __ldcg(pr + Rec::kS + nn * 8 + 2 * t4 + cc) : 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < kChunks; ++i)
-            ov[b][i][nn] = have ? __ldcg(reinterpret_cast<const uint2*>(pr) + (i * NT + nn) * 32 + lane) : make_uint2(0u, 0u);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-        for (int nn = 0; nn < NT; ++nn) {
-          float w[2], a[2];
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const float mn = fmaxf(M[nn][cc], mv[b][nn][cc]);
-            a[cc] = fast_exp2(M[nn][cc] - mn);
-            w[cc] = fast_exp2(mv[b][nn][cc] - mn) * lv[b][nn][cc];
-            L[nn][cc] = L[nn][cc] * a[cc] + w[cc];
-            M[nn][cc] = mn;
-            w[cc] *= sv[b][nn][cc];
-          }
-#pragma unroll
-          for (int i = 0; i < kChunks; ++i) {
-            const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&ov[b][i][nn].x));
-            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&ov[b][i][nn].y));
-            O[i][nn][0] = O[i][nn][0] * a[0] + lo.x * w[0];
-            O[i][nn][1] = O[i][nn][1] * a[1] + lo.y * w[1];
-            O[i][nn][2] = O[i][nn][2] * a[0] + hi.x * w[0];
-            O[i][nn][3] = O[i][nn][3] * a[1] + hi.y * w[1];
-          }
-        }
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+  }
+  __syncthreads();
+  for (int j = 0; j < opens; ++j) {
+    if (!last_of[j]) continue;
+    for (int item = warp; item < kItems; item += W) {
+      Merge<Joined, NT, true> mg;
+      mg.template run<4>(open_c1[j] - open_c0[j] + 1, item, lane, [&](int k) -> const float* {
+        const int c = open_c0[j] + k;
+        const int slot = open_cb[j] <= r.start(c * W) ? 0 : 1;
+        return p.joined + (((size_t)head * gridDim.x + c) * 2 + slot) * Joined::kFloats;
+      });
+      write_item(open_v[j], item, mg.o, mg.l);
     }
-#pragma unroll
-    for (int nn = 0; nn < NT; ++nn) {
-      L[nn][0] = L[nn][0] > 0.f ? 1.f / L[nn][0] : 0.f;
-      L[nn][1] = L[nn][1] > 0.f ? 1.f / L[nn][1] : 0.f;
-    }
-    write_out(virtual_of<NC>(p, pend_v[j]), O, L);
   }
 }
 
@@ -851,10 +964,13 @@ struct Fp8Plan {
 
 template <typename T, int D, int NT, int S, int W>
 Fp8Plan make_fp8_plan() {
-  static_assert(W <= 8 && NT <= 4 && D <= 128, "the workspace has room for these");
+  static_assert(NT <= 4 && D <= 128, "the workspace has room for these");
   Fp8Plan pl;
   pl.fn = reinterpret_cast<const void*>(&paged_rows_fp8<T, D, NT, S, W>);
-  pl.smem = W * S * 4 * kSub * D + (NT > 2 ? W * (D / 16) * NT * 32 * 8 : 0) + W * S * 8 + 1024;
+  using Rec = Fp8Record<D, NT, std::is_same<T, __half>::value && NT <= 2>;
+  pl.smem = W * S * 4 * kSub * D + (NT > 2 ? W * (D / 16) * NT * 32 * 8 : 0) + W * Rec::kFloats * 4 + W * S * 8 + 1024;
+  static_assert(W * S * 4 * kSub * D + (NT > 2 ? W * (D / 16) * NT * 32 * 8 : 0) + W * Rec::kFloats * 4 + W * S * 8 +
+                        1024 + W * 64 + 64 <= 227 * 1024, "shared memory of an SM");
   pl.warps = W;
   pl.columns = NT * 8;
   return pl;
@@ -863,9 +979,9 @@ Fp8Plan make_fp8_plan() {
 template <typename T>
 bool select_fp8_plan(int head_dim, int columns, Fp8Plan& pl) {
   if (head_dim == 128)
-    pl = columns <= 8 ? make_fp8_plan<T, 128, 1, 3, 8>()
-         : columns <= 16 ? make_fp8_plan<T, 128, 2, 3, 8>()
-                         : make_fp8_plan<T, 128, 4, 2, 8>();
+    pl = columns <= 8 ? make_fp8_plan<T, 128, 1, 2, 8>()
+         : columns <= 16 ? make_fp8_plan<T, 128, 2, 2, 8>()
+                         : make_fp8_plan<T, 128, 4, 2, 6>();
   else if (head_dim == 64)
     pl = columns <= 8 ? make_fp8_plan<T, 64, 1, 4, 8>()
          : columns <= 16 ? make_fp8_plan<T, 64, 2, 4, 8>()
@@ -886,12 +1002,11 @@ int64_t fp8_ctas(int num_kv_heads) {
 // that followed the call's own records, one buffer used for calls of one and of five rows in
 // turn would find records where it looks for zeroed counters.)
 constexpr int kMostColumns = 32;   // per virtual sequence
-constexpr int kMostUnits = 8;      // warps per CTA of any plan
 constexpr int kRowColumns = 64;    // columns per sequence that calls here have at most
 
 size_t records_bytes(int num_kv_heads) {
   const int64_t ctas = num_kv_heads > b2p_host::sm_count() ? num_kv_heads : b2p_host::sm_count();
-  return (size_t)ctas * kMostUnits * 2 * Fp8Record<128, kMostColumns / 8>::kFloats * 4;
+  return (size_t)ctas * 2 * Fp8Record<128, kMostColumns / 8, true>::kFloats * 4;
 }
 
 int column_groups(const Fp8Plan& pl, int group, int max_q_len) {
@@ -945,6 +1060,9 @@ int b2p_rows_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, con
       if (i < 32) ready[dev][i] = pl.fn;
     }
   }
+  // 31 bits count the tiles of a KV head
+  const int64_t width_tiles = (block_table_stride * block_size + kTile - 1) / kTile;
+  if (width_tiles * num_seqs * column_groups(pl, group, max_q_len) > 0x7fffffffLL) return B2P_EUNSUPPORTED;
   CUtensorMap kmap, vmap;
   int rc = b2p_host::fp8_pool_tensor_map(&kmap, key_cache, num_layers, num_slots, num_kv_heads, head_dim);
   if (rc != B2P_OK) return rc;
@@ -966,6 +1084,9 @@ int b2p_rows_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, con
   p.max_q_len = max_q_len;
   p.groups_per_seq = column_groups(pl, group, max_q_len);
   p.group = group;
+  p.group_inv = (65536 + group - 1) / group;
+  const int64_t reach = block_table_stride * block_size;
+  p.most_keys = (int)(reach < 0x7fffff00LL ? reach : 0x7fffff00LL);
   p.layer = (int)layer_index;
   p.block_size = block_size;
   p.hkv = num_kv_heads;
@@ -973,7 +1094,7 @@ int b2p_rows_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, con
   p.k_scales = key_scales + layer_index * p.num_blocks * num_kv_heads;
   p.v_scales = value_scales + layer_index * p.num_blocks * num_kv_heads;
   p.scale_log2 = scale * kLog2e;
-  p.partials = static_cast<float*>(workspace);
+  p.joined = static_cast<float*>(workspace);
   p.counters = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + records_bytes(num_kv_heads));
   p.err = err_flag;
   cudaLaunchConfig_t cfg = {};

@@ -382,53 +382,84 @@ def lm_head_argmax(
 FP8_DTYPE = torch.float8_e4m3fn
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """Launch on ``device``'s current stream, whichever device is current."""
+# The current stream's handle and the current device's index without torch.cuda's wrappers: the
+# calls below take a few microseconds on the host, of which those two would be one.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call(name: str, index: int, *args) -> None:
+    """Launch on CUDA device ``index``'s current stream, whichever device is current."""
     fn = getattr(_lib.load(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = fn(*args, _stream(device))
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
-    _lib.check(rc, name)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _on(device: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            _require_cuda(name, t)
-            raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+def _index_of(name: str, t: torch.Tensor) -> int:
+    """CUDA device index of t."""
+    index = t.get_device()
+    if index < 0:
+        _require_cuda(name, t)
+    return index
 
 
-def _err_flag(err_flag: torch.Tensor | None) -> int | None:
+def _on(index: int, name: str, t: torch.Tensor) -> None:
+    if t.get_device() != index:
+        _require_cuda(name, t)
+        raise ValueError(f"{name} is on {t.device}, the other tensors on cuda:{index}")
+
+
+def _vector(index: int, name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
+    if t.dtype is not dtype or not t.is_contiguous():
+        _require_cuda(name, t)
+        raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor")
+    _on(index, name, t)
+
+
+def _err_flag(index: int, err_flag: torch.Tensor | None) -> int | None:
     if err_flag is None:
         return None
-    _int32("err_flag", err_flag)
+    _vector(index, "err_flag", err_flag, torch.int32)
     return err_flag.data_ptr()
 
 
 def _check_fp8_pool(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: torch.Tensor,
-                    value_scales: torch.Tensor, block_size: int) -> None:
-    _check_pool(key_cache, value_cache)
-    if key_cache.dtype != FP8_DTYPE:
-        raise ValueError(f"an 8-bit pool must be {FP8_DTYPE} (got {key_cache.dtype})")
-    layers, slots, hkv, _ = key_cache.shape
-    if block_size <= 0 or slots % block_size:
+                    value_scales: torch.Tensor, block_size: int) -> tuple[int, torch.Size]:
+    """(device index, pool shape) of a valid 8-bit pool."""
+    index = _index_of("key_cache", key_cache)
+    shape = key_cache.shape
+    if value_cache.shape != shape or len(shape) != 4:
+        raise ValueError("key_cache/value_cache must both be [layers, slots, kv_heads, head_dim]")
+    if key_cache.dtype is not FP8_DTYPE or value_cache.dtype is not FP8_DTYPE:
+        raise ValueError(f"an 8-bit pool must be {FP8_DTYPE} (got {key_cache.dtype}, {value_cache.dtype})")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise ValueError("key_cache/value_cache must be contiguous")
+    _on(index, "value_cache", value_cache)
+    if block_size <= 0 or shape[1] % block_size:
         raise ValueError("the pool's slots must be a multiple of block_size")
-    shape = (layers, slots // block_size, hkv)
-    for name, t in (("key_scales", key_scales), ("value_scales", value_scales)):
-        if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous float32 tensor of shape {shape}")
-    _on(key_cache.device, value_cache=value_cache, key_scales=key_scales, value_scales=value_scales)
+    want = (shape[0], shape[1] // block_size, shape[2])
+    if key_scales.shape != want or value_scales.shape != want:
+        raise ValueError(f"key_scales/value_scales must have shape {want}")
+    _vector(index, "key_scales", key_scales, torch.float32)
+    _vector(index, "value_scales", value_scales, torch.float32)
+    return index, shape
 
 
-def _check_tables(device: torch.device, num_seqs: int, block_tables: torch.Tensor,
-                  context_lens: torch.Tensor) -> None:
-    _int32("block_tables", block_tables)
-    _int32("context_lens", context_lens)
-    if block_tables.dim() != 2 or block_tables.shape[0] < num_seqs or context_lens.numel() < num_seqs:
+def _check_tables(index: int, num_seqs: int, block_tables: torch.Tensor,
+                  context_lens: torch.Tensor) -> int:
+    """The block tables' width."""
+    _vector(index, "block_tables", block_tables, torch.int32)
+    _vector(index, "context_lens", context_lens, torch.int32)
+    shape = block_tables.shape
+    if len(shape) != 2 or shape[0] < num_seqs or context_lens.numel() < num_seqs or num_seqs < 0:
         raise ValueError("block_tables/context_lens must cover every sequence")
-    _on(device, block_tables=block_tables, context_lens=context_lens)
+    return shape[1]
 
 
 def kv_write_fp8(
@@ -458,25 +489,28 @@ def kv_write_fp8(
     rounds the rows before it to the new scale where that grows. A non-finite row makes the
     scale NaN. Two sequences of one call must not append to the same block.
     """
-    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
-    dev = key_cache.device
+    index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
+                                                     value_scales, block_size)
     n = cu_seqlens_q.numel() - 1
-    _int32("cu_seqlens_q", cu_seqlens_q)
-    _check_tables(dev, n, block_tables, context_lens)
-    _on(dev, cu_seqlens_q=cu_seqlens_q, keys=keys, values=values, err_flag=err_flag)
-    layers, slots, hkv, d = key_cache.shape
-    if keys.shape != values.shape or keys.dim() != 3 or tuple(keys.shape[1:]) != (hkv, d):
+    _vector(index, "cu_seqlens_q", cu_seqlens_q, torch.int32)
+    width = _check_tables(index, n, block_tables, context_lens)
+    _on(index, "keys", keys)
+    _on(index, "values", values)
+    shape = keys.shape
+    if values.shape != shape or len(shape) != 3 or shape[1] != hkv or shape[2] != d:
         raise ValueError(f"keys/values must have shape (tokens, {hkv}, {d})")
-    if keys.dtype != values.dtype:
+    if keys.dtype is not values.dtype:
         raise ValueError("keys/values dtypes differ")
-    kt, kh = _tok_head_strides("keys", keys)
-    vt, vh = _tok_head_strides("values", values)
-    _call("b2p_kv_write_fp8", dev, keys.data_ptr(), kt, kh, values.data_ptr(), vt, vh,
+    kt, kh, kd = keys.stride()
+    vt, vh, vd = values.stride()
+    if kd != 1 or vd != 1:
+        raise ValueError("keys/values must have a contiguous head_dim")
+    _call("b2p_kv_write_fp8", index, keys.data_ptr(), kt, kh, values.data_ptr(), vt, vh,
           key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
-          value_scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-          cu_seqlens_q.data_ptr(), context_lens.data_ptr(), n, keys.shape[0], max_q_len,
+          value_scales.data_ptr(), block_tables.data_ptr(), width,
+          cu_seqlens_q.data_ptr(), context_lens.data_ptr(), n, shape[0], max_q_len,
           layer_index, layers, slots, hkv, d, block_size, dtype_code(keys.dtype),
-          _err_flag(err_flag))
+          _err_flag(index, err_flag))
 
 
 def kv_read_fp8(
@@ -492,19 +526,17 @@ def kv_read_fp8(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows of the given slots (int32) as values of ``dtype``: (keys, values), each
     (rows, kv_heads, head_dim). Negative slots give zero rows."""
-    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
-    dev = key_cache.device
-    _int32("slot_mapping", slot_mapping)
-    _on(dev, slot_mapping=slot_mapping, err_flag=err_flag)
+    index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
+                                                     value_scales, block_size)
+    _vector(index, "slot_mapping", slot_mapping, torch.int32)
     code = dtype_code(dtype)
-    layers, slots, hkv, d = key_cache.shape
     n = slot_mapping.numel()
-    keys = torch.empty((n, hkv, d), dtype=dtype, device=dev)
+    keys = torch.empty((n, hkv, d), dtype=dtype, device=key_cache.device)
     values = torch.empty_like(keys)
-    _call("b2p_kv_read_fp8", dev, key_cache.data_ptr(), value_cache.data_ptr(),
+    _call("b2p_kv_read_fp8", index, key_cache.data_ptr(), value_cache.data_ptr(),
           key_scales.data_ptr(), value_scales.data_ptr(), slot_mapping.data_ptr(), n,
           keys.data_ptr(), values.data_ptr(), layer_index, layers, slots, hkv, d, block_size, code,
-          _err_flag(err_flag))
+          _err_flag(index, err_flag))
     return keys, values
 
 
@@ -522,24 +554,30 @@ def make_fp8_workspace(max_seqs: int, num_q_heads: int, num_kv_heads: int, head_
     return torch.zeros(max(n, 16), dtype=torch.uint8, device=device)
 
 
-def _check_fp8_query(q: torch.Tensor, key_cache: torch.Tensor, out: torch.Tensor | None):
-    if q.dim() != 3 or q.shape[2] != key_cache.shape[3]:
+def _fp8_query(index: int, head_dim: int, q: torch.Tensor, out: torch.Tensor | None):
+    """(dtype code, out, q's and out's token and head strides) of a valid query."""
+    _on(index, "q", q)
+    if q.dim() != 3 or q.shape[2] != head_dim:
         raise ValueError("q must be (rows, num_q_heads, head_dim) with the pool's head_dim")
     code = dtype_code(q.dtype)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must have q's shape and dtype")
-    return code, out
+    else:
+        _on(index, "out", out)
+        if out.shape != q.shape or out.dtype is not q.dtype:
+            raise ValueError("out must have q's shape and dtype")
+    qt, qh, qd = q.stride()
+    ot, oh, od = out.stride()
+    if qd != 1 or od != 1:
+        raise ValueError("q and out must have a contiguous head_dim")
+    return code, out, qt, qh, ot, oh
 
 
-def _fp8_workspace(workspace: torch.Tensor | None, n: int, hq: int, hkv: int, d: int,
-                   device: torch.device, max_q_len: int) -> torch.Tensor:
+def _fp8_workspace(index: int, workspace: torch.Tensor | None, n: int, hq: int, hkv: int, d: int,
+                   max_q_len: int) -> torch.Tensor:
     if workspace is None:
-        return make_fp8_workspace(n, hq, hkv, d, device, max_q_len)
-    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise ValueError("workspace must be a contiguous uint8 tensor")
-    _on(device, workspace=workspace)
+        return make_fp8_workspace(n, hq, hkv, d, torch.device("cuda", index), max_q_len)
+    _vector(index, "workspace", workspace, torch.uint8)
     return workspace
 
 
@@ -562,21 +600,17 @@ def paged_decode_fp8(
 
     q: (num_seqs, num_q_heads, head_dim) in bf16, f16 or fp32; returns out of the same shape.
     """
-    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
-    dev = key_cache.device
-    code, out = _check_fp8_query(q, key_cache, out)
-    n, hq, d = q.shape
-    layers, slots, hkv, _ = key_cache.shape
-    _check_tables(dev, n, block_tables, context_lens)
-    _on(dev, q=q, out=out, err_flag=err_flag)
-    qt, qh = _tok_head_strides("q", q)
-    ot, oh = _tok_head_strides("out", out)
-    workspace = _fp8_workspace(workspace, n, hq, hkv, d, dev, 1)
-    _call("b2p_paged_decode_fp8", dev, q.data_ptr(), qt, qh, key_cache.data_ptr(),
+    index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
+                                                     value_scales, block_size)
+    code, out, qt, qh, ot, oh = _fp8_query(index, d, q, out)
+    n, hq, _ = q.shape
+    width = _check_tables(index, n, block_tables, context_lens)
+    workspace = _fp8_workspace(index, workspace, n, hq, hkv, d, 1)
+    _call("b2p_paged_decode_fp8", index, q.data_ptr(), qt, qh, key_cache.data_ptr(),
           value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
-          layers, slots, block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(),
-          n, hq, hkv, d, block_size, float(scale), out.data_ptr(), ot, oh, workspace.data_ptr(),
-          workspace.numel(), code, _err_flag(err_flag))
+          layers, slots, block_tables.data_ptr(), width, context_lens.data_ptr(), n, hq, hkv, d,
+          block_size, scale, out.data_ptr(), ot, oh, workspace.data_ptr(), workspace.numel(), code,
+          _err_flag(index, err_flag))
     return out
 
 
@@ -606,27 +640,23 @@ def paged_prefill_fp8(
     owns are left alone in out. Calls of many rows widen the histories into a 16-bit copy of
     ``num_seqs * block_tables.shape[1]`` blocks of one layer, allocated for the call.
     """
-    _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
-    dev = key_cache.device
-    code, out = _check_fp8_query(q, key_cache, out)
-    total_q, hq, d = q.shape
-    layers, slots, hkv, _ = key_cache.shape
+    index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
+                                                     value_scales, block_size)
+    code, out, qt, qh, ot, oh = _fp8_query(index, d, q, out)
+    total_q, hq, _ = q.shape
     n = cu_seqlens_q.numel() - 1
-    _int32("cu_seqlens_q", cu_seqlens_q)
-    _check_tables(dev, n, block_tables, context_lens)
-    _on(dev, q=q, out=out, cu_seqlens_q=cu_seqlens_q, err_flag=err_flag)
-    qt, qh = _tok_head_strides("q", q)
-    ot, oh = _tok_head_strides("out", out)
-    workspace = _fp8_workspace(workspace, n, hq, hkv, d, dev, max_q_len)
-    size = int(_lib.load().b2p_paged_prefill_fp8_scratch_size(
-        n, block_tables.stride(0), hq, hkv, d, block_size, max_q_len, code))
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _call("b2p_paged_prefill_fp8", dev, q.data_ptr(), qt, qh, key_cache.data_ptr(),
+    _vector(index, "cu_seqlens_q", cu_seqlens_q, torch.int32)
+    width = _check_tables(index, n, block_tables, context_lens)
+    workspace = _fp8_workspace(index, workspace, n, hq, hkv, d, max_q_len)
+    size = _lib.load().b2p_paged_prefill_fp8_scratch_size(n, width, hq, hkv, d, block_size,
+                                                          max_q_len, code)
+    scratch = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    _call("b2p_paged_prefill_fp8", index, q.data_ptr(), qt, qh, key_cache.data_ptr(),
           value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
-          layers, slots, block_tables.data_ptr(), block_tables.stride(0), cu_seqlens_q.data_ptr(),
-          context_lens.data_ptr(), n, total_q, max_q_len, hq, hkv, d, block_size, float(scale),
+          layers, slots, block_tables.data_ptr(), width, cu_seqlens_q.data_ptr(),
+          context_lens.data_ptr(), n, total_q, max_q_len, hq, hkv, d, block_size, scale,
           out.data_ptr(), ot, oh, workspace.data_ptr(), workspace.numel(), _ptr(scratch), size,
-          code, _err_flag(err_flag))
+          code, _err_flag(index, err_flag))
     return out
 
 
@@ -635,15 +665,14 @@ def _drafts_out(n: int, max_drafts: int, device: torch.device):
             torch.empty(n, dtype=torch.int32, device=device))
 
 
-def _check_drafts(device: torch.device, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor,
+def _check_drafts(index: int, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor,
                   max_drafts: int) -> int:
-    _int32("cu_drafts", cu_drafts)
-    if draft_tokens.dim() != 1 or draft_tokens.dtype != torch.int64 or not draft_tokens.is_contiguous():
-        raise ValueError("draft_tokens must be a contiguous int64 vector")
-    if max_drafts < 0 or cu_drafts.numel() < 1:
+    _vector(index, "cu_drafts", cu_drafts, torch.int32)
+    _vector(index, "draft_tokens", draft_tokens, torch.int64)
+    n = cu_drafts.numel() - 1
+    if max_drafts < 0 or n < 0:
         raise ValueError("max_drafts must not be negative and cu_drafts needs an entry")
-    _on(device, draft_tokens=draft_tokens, cu_drafts=cu_drafts)
-    return cu_drafts.numel() - 1
+    return n
 
 
 def verify_drafts(
@@ -667,30 +696,35 @@ def verify_drafts(
     [0, 1). Returns (tokens, accepted): int64 (num_seqs, max_drafts + 1), the standing drafts, then
     the drawn token, then -1; and int32 (num_seqs,), how many drafts stand.
     """
-    _require_cuda("target_probs", target_probs)
-    dev = target_probs.device
-    n = _check_drafts(dev, draft_tokens, cu_drafts, max_drafts)
+    index = _index_of("target_probs", target_probs)
+    n = _check_drafts(index, draft_tokens, cu_drafts, max_drafts)
     total = draft_tokens.numel()
-    code = dtype_code(target_probs.dtype)
-    if target_probs.dim() != 2 or target_probs.shape[0] != total + n or target_probs.stride(1) != 1:
-        raise ValueError(f"target_probs must be ({total + n}, vocab) with contiguous rows")
-    if draft_probs is not None and (
-            draft_probs.dim() != 2 or tuple(draft_probs.shape) != (total, target_probs.shape[1])
-            or draft_probs.dtype != target_probs.dtype or draft_probs.stride(1) != 1):
-        raise ValueError("draft_probs must be (drafts, vocab) in target_probs' dtype with "
-                         "contiguous rows")
-    for name, t, want in (("accept_draws", accept_draws, total), ("sample_draws", sample_draws, n)):
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != want:
-            raise ValueError(f"{name} must be a contiguous float32 tensor of {want} entries")
-    _on(dev, draft_probs=draft_probs, accept_draws=accept_draws, sample_draws=sample_draws,
-        err_flag=err_flag)
-    tokens, accepted = _drafts_out(n, max_drafts, dev)
-    with_q = draft_probs is not None and total > 0
-    _call("b2p_verify_drafts", dev, target_probs.data_ptr(), target_probs.stride(0),
-          draft_probs.data_ptr() if with_q else None, draft_probs.stride(0) if with_q else 0,
+    dtype = target_probs.dtype
+    code = dtype_code(dtype)
+    if target_probs.dim() != 2 or target_probs.shape[0] != total + n:
+        raise ValueError(f"target_probs must be ({total + n}, vocab)")
+    vocab = target_probs.shape[1]
+    t_row, one = target_probs.stride()
+    if one != 1 and vocab > 1:
+        raise ValueError("target_probs must have contiguous rows")
+    q_ptr, q_row = None, 0
+    if draft_probs is not None:
+        _on(index, "draft_probs", draft_probs)
+        if draft_probs.shape != (total, vocab) or draft_probs.dtype is not dtype:
+            raise ValueError(f"draft_probs must be ({total}, {vocab}) in target_probs' dtype")
+        q_row, one = draft_probs.stride()
+        if one != 1 and vocab > 1:
+            raise ValueError("draft_probs must have contiguous rows")
+        q_ptr = draft_probs.data_ptr() or None  # no drafts: an empty tensor
+    _vector(index, "accept_draws", accept_draws, torch.float32)
+    _vector(index, "sample_draws", sample_draws, torch.float32)
+    if accept_draws.numel() != total or sample_draws.numel() != n:
+        raise ValueError(f"accept_draws must have {total} entries and sample_draws {n}")
+    tokens, accepted = _drafts_out(n, max_drafts, target_probs.device)
+    _call("b2p_verify_drafts", index, target_probs.data_ptr(), t_row, q_ptr, q_row,
           draft_tokens.data_ptr(), cu_drafts.data_ptr(), accept_draws.data_ptr(),
-          sample_draws.data_ptr(), n, total, max_drafts, target_probs.shape[1], code,
-          tokens.data_ptr(), tokens.stride(0), accepted.data_ptr(), _err_flag(err_flag))
+          sample_draws.data_ptr(), n, total, max_drafts, vocab, code, tokens.data_ptr(),
+          max_drafts + 1, accepted.data_ptr(), _err_flag(index, err_flag))
     return tokens, accepted
 
 
@@ -703,35 +737,36 @@ def verify_drafts_greedy(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The greedy form of ``verify_drafts``: target_ids (int64, drafts + num_seqs) holds the
     arg-max of each target row (what ``lm_head_argmax`` gives); drafts stand while they equal it."""
-    _require_cuda("target_ids", target_ids)
-    dev = target_ids.device
-    n = _check_drafts(dev, draft_tokens, cu_drafts, max_drafts)
+    index = _index_of("target_ids", target_ids)
+    n = _check_drafts(index, draft_tokens, cu_drafts, max_drafts)
     total = draft_tokens.numel()
-    if target_ids.dtype != torch.int64 or not target_ids.is_contiguous() or \
-            target_ids.numel() != total + n:
-        raise ValueError(f"target_ids must be a contiguous int64 tensor of {total + n} entries")
-    _on(dev, err_flag=err_flag)
-    tokens, accepted = _drafts_out(n, max_drafts, dev)
-    _call("b2p_verify_drafts_greedy", dev, target_ids.data_ptr(), draft_tokens.data_ptr(),
-          cu_drafts.data_ptr(), n, total, max_drafts, tokens.data_ptr(), tokens.stride(0),
-          accepted.data_ptr(), _err_flag(err_flag))
+    _vector(index, "target_ids", target_ids, torch.int64)
+    if target_ids.numel() != total + n:
+        raise ValueError(f"target_ids must have {total + n} entries")
+    tokens, accepted = _drafts_out(n, max_drafts, target_ids.device)
+    _call("b2p_verify_drafts_greedy", index, target_ids.data_ptr(), draft_tokens.data_ptr(),
+          cu_drafts.data_ptr(), n, total, max_drafts, tokens.data_ptr(), max_drafts + 1,
+          accepted.data_ptr(), _err_flag(index, err_flag))
     return tokens, accepted
 
 
 def _check_pages(key_cache: torch.Tensor, value_cache: torch.Tensor, block_size: int,
-                 key_scales: torch.Tensor | None, value_scales: torch.Tensor | None) -> None:
-    if key_cache.dtype == FP8_DTYPE:
+                 key_scales: torch.Tensor | None, value_scales: torch.Tensor | None
+                 ) -> tuple[int, torch.Size]:
+    """(device index, pool shape) of a valid pool of any dtype."""
+    if key_cache.dtype is FP8_DTYPE:
         if key_scales is None or value_scales is None:
             raise ValueError("an 8-bit pool needs its key_scales and value_scales")
-        _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
-        return
+        return _check_fp8_pool(key_cache, value_cache, key_scales, value_scales, block_size)
     _check_pool(key_cache, value_cache)
     dtype_code(key_cache.dtype)
     if key_scales is not None or value_scales is not None:
         raise ValueError("only an 8-bit pool has scales")
     if block_size <= 0 or key_cache.shape[1] % block_size:
         raise ValueError("the pool's slots must be a multiple of block_size")
-    _on(key_cache.device, value_cache=value_cache)
+    index = key_cache.get_device()
+    _on(index, "value_cache", value_cache)
+    return index, key_cache.shape
 
 
 def copy_blocks(
@@ -747,17 +782,16 @@ def copy_blocks(
     """K9: copy block src_blocks[i] to block dst_blocks[i] in every layer of K and V (and of the
     scales of an 8-bit pool). int32 CUDA vectors; a pair with a negative id is skipped. Targets
     must be distinct, and none of them a source of the same call."""
-    _check_pages(key_cache, value_cache, block_size, key_scales, value_scales)
-    _int32("src_blocks", src_blocks)
-    _int32("dst_blocks", dst_blocks)
-    if src_blocks.numel() != dst_blocks.numel():
+    index, (layers, slots, hkv, d) = _check_pages(key_cache, value_cache, block_size, key_scales,
+                                                  value_scales)
+    _vector(index, "src_blocks", src_blocks, torch.int32)
+    _vector(index, "dst_blocks", dst_blocks, torch.int32)
+    pairs = src_blocks.numel()
+    if dst_blocks.numel() != pairs:
         raise ValueError("src_blocks and dst_blocks must have one entry per pair")
-    dev = key_cache.device
-    _on(dev, src_blocks=src_blocks, dst_blocks=dst_blocks, err_flag=err_flag)
-    layers, slots, hkv, d = key_cache.shape
-    _call("b2p_copy_blocks", dev, key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scales),
-          _ptr(value_scales), src_blocks.data_ptr(), dst_blocks.data_ptr(), src_blocks.numel(),
-          layers, slots, hkv, d, key_cache.element_size(), block_size, _err_flag(err_flag))
+    _call("b2p_copy_blocks", index, key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scales),
+          _ptr(value_scales), src_blocks.data_ptr(), dst_blocks.data_ptr(), pairs, layers, slots,
+          hkv, d, key_cache.element_size(), block_size, _err_flag(index, err_flag))
 
 
 def compact_blocks(
@@ -776,20 +810,17 @@ def compact_blocks(
     live block and -1 for the others, and int32 (1,). Live blocks already in place stay; the
     j-th of the others, in ascending order, goes to the j-th free block. A block that no row names
     counts as free: pass every table that is in use."""
-    _check_pages(key_cache, value_cache, block_size, key_scales, value_scales)
-    dev = key_cache.device
+    index, (layers, slots, hkv, d) = _check_pages(key_cache, value_cache, block_size, key_scales,
+                                                  value_scales)
     n = context_lens.numel()
-    _check_tables(dev, n, block_tables, context_lens)
-    _on(dev, err_flag=err_flag)
-    layers, slots, hkv, d = key_cache.shape
-    blocks = slots // block_size
-    size = int(_lib.load().b2p_compact_blocks_workspace_size(blocks))
+    width = _check_tables(index, n, block_tables, context_lens)
+    dev, blocks = key_cache.device, slots // block_size
+    size = _lib.load().b2p_compact_blocks_workspace_size(blocks)
     workspace = torch.empty(size, dtype=torch.uint8, device=dev)
     new_ids = torch.empty(blocks, dtype=torch.int32, device=dev)
     num_live = torch.empty(1, dtype=torch.int32, device=dev)
-    _call("b2p_compact_blocks", dev, key_cache.data_ptr(), value_cache.data_ptr(),
-          _ptr(key_scales), _ptr(value_scales), block_tables.data_ptr(), block_tables.stride(0),
-          block_tables.shape[1], context_lens.data_ptr(), n, layers, slots, hkv, d,
+    _call("b2p_compact_blocks", index, key_cache.data_ptr(), value_cache.data_ptr(),
+          _ptr(key_scales), _ptr(value_scales), block_tables.data_ptr(), width, width, context_lens.data_ptr(), n, layers, slots, hkv, d,
           key_cache.element_size(), block_size, new_ids.data_ptr(), num_live.data_ptr(),
-          workspace.data_ptr(), size, _err_flag(err_flag))
+          workspace.data_ptr(), size, _err_flag(index, err_flag))
     return new_ids, num_live
