@@ -7,7 +7,9 @@
 // arithmetic, so the instructions per byte are what the design saves on.
 //
 //  * A sequence's columns are its (row, query head of the GQA group) pairs, q_len * G of them;
-//    up to 8 * NT go through one pass over its keys ("virtual sequence"), more in further ones.
+//    up to 8 * NT go through one pass over its keys ("virtual sequence"), more in further ones,
+//    which mostly find the codes in L2. NT is 2 at most: with 4 (one pass of 32 columns) O alone
+//    takes 128 registers and the loop spills; 128 sequences of 1 to 6 rows took 119 us against 71.
 //  * Work = per KV head the flattened list of 32-token tiles of all virtual sequences, cut into
 //    equal ranges, one per warp (stream-K at warp granularity). A warp owns a ring of S stages
 //    that its lane 0 fills by TMA (two 16-token boxes of K and of V per stage) and resolves the
@@ -84,20 +86,19 @@ __device__ __forceinline__ int row_of(const Fp8Params& p, int col) {
 template <int NC>
 __device__ __forceinline__ Virtual virtual_of(const Fp8Params& p, int v) {
   Virtual t;
-  if (p.cu == nullptr) {
-    t.seq = t.row0 = v;
+  t.seq = p.groups_per_seq == 1 ? v : v / p.groups_per_seq;
+  t.col0 = (v - t.seq * p.groups_per_seq) * NC;
+  t.ctx = min(__ldg(p.ctx + t.seq), p.most_keys);
+  if (p.cu == nullptr) {  // one row per sequence
+    t.row0 = t.seq;
     t.qlen = 1;
-    t.ctx = t.keys = min(max(0, __ldg(p.ctx + v)), p.most_keys);
-    t.col0 = 0;
-    t.cols = p.group;
+    t.cols = min(NC, p.group - t.col0);
+    t.keys = max(0, t.ctx);
     return t;
   }
-  t.seq = p.groups_per_seq == 1 ? v : v / p.groups_per_seq;
   t.row0 = __ldg(p.cu + t.seq);
   const int end = __ldg(p.cu + t.seq + 1);
-  t.ctx = min(__ldg(p.ctx + t.seq), p.most_keys);
   t.qlen = end - t.row0;
-  t.col0 = (v - t.seq * p.groups_per_seq) * NC;
   if (t.qlen <= 0 || t.qlen > p.max_q_len || t.row0 < 0 || end > p.num_rows) t.qlen = 0;
   t.cols = min(NC, t.qlen * p.group - t.col0);
   if (t.cols <= 0) {
@@ -114,24 +115,24 @@ __device__ __forceinline__ int tiles_of(const Fp8Params& p, int v, int nv) {
   return v < nv ? (virtual_of<NC>(p, v).keys + kTile - 1) / kTile : 0;
 }
 
-// A partial result: O^T / (l s) in MMA fragment order, then per column m_x, the sum l and the
-// scale s = max_d |O / l|. For bf16 output O is kept in f16 (2^-11 of the column's largest
-// value, against an output step of 2^-8). For f16 output it is kept in fp32 (in f16 it would
-// round once more as coarsely as the output), but with four column tiles, whose fp32 records
-// would not fit in shared memory. CTAs' records are fp32.
+// A partial result: O^T / (l s) in MMA fragment order, then per column the logarithm of its
+// weight, m_x + log2(l) (kNoMax: it saw nothing), and the scale s = max_d |O / l|. For bf16
+// output O is kept in f16 (2^-11 of the column's largest value, against an output step of 2^-8);
+// for f16 output it is kept in fp32 (in f16 it would round once more as coarsely as the output).
+// CTAs' records are fp32.
 template <int D, int NT, bool kWide>
 struct Fp8Record {
-  static constexpr int kOBytes = (D / 16) * NT * 32 * (kWide ? 16 : 8);
-  static constexpr int kM = kOBytes / 4;  // float index of the references
-  static constexpr int kL = kM + NT * 8;  // ... of the sums
-  static constexpr int kS = kL + NT * 8;  // ... of the scales
-  static constexpr int kFloats = kS + NT * 8;
+  static constexpr int kStats = (D / 16) * NT * 32 * (kWide ? 16 : 8) / 4;  // float index
+  static constexpr int kFloats = kStats + NT * 8 * 2;
 
   __device__ static void put(float* rec, int item, int lane, float a, float b, float c, float d) {
     if constexpr (kWide)
       reinterpret_cast<float4*>(rec)[item * 32 + lane] = make_float4(a, b, c, d);
     else
       reinterpret_cast<uint2*>(rec)[item * 32 + lane] = make_uint2(pack2<__half>(a, b), pack2<__half>(c, d));
+  }
+  __device__ static void put_stats(float* rec, int c, float weight, float scale) {
+    *reinterpret_cast<float2*>(rec + kStats + 2 * c) = make_float2(weight, scale);
   }
   template <bool kGlobal>  // another CTA's record (L2), or this CTA's in shared memory
   __device__ static float4 get(const float* rec, int item, int lane) {
@@ -146,48 +147,76 @@ struct Fp8Record {
       return make_float4(lo.x, lo.y, hi.x, hi.y);
     }
   }
-  template <bool kGlobal>  // the two columns c, c + 1 of field `at`
-  __device__ static float2 pair(const float* rec, int at, int c) {
-    const float2* x = reinterpret_cast<const float2*>(rec + at + c);
-    return kGlobal ? __ldcg(x) : *x;
+  template <bool kGlobal>  // (weight, scale) of columns c and c + 1
+  __device__ static float4 stats(const float* rec, int c) {
+    const float4* at = reinterpret_cast<const float4*>(rec + kStats + 2 * c);
+    return kGlobal ? __ldcg(at) : *at;
   }
 };
 
-// One fragment (item = chunk * NT + nn; a lane's four values of two columns) of records merged.
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// log2 weight of a column whose sum is l against m.
+__device__ __forceinline__ float weight_of(float m, float l) { return l == 0.f ? kNoMax : m + log2_fast(l); }
+
+// One fragment (item = chunk * NT + nn; a lane's four values of two columns) of records merged:
+// o = sum_k 2^(w_k - top) s_k O_k, l = sum_k 2^(w_k - top). A CTA runs two warps per scheduler at
+// this point, so instructions count: some twenty per record.
 template <typename Rec, int NT, bool kGlobal>
 struct Merge {
-  float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
-  float o[4] = {0.f, 0.f, 0.f, 0.f};  // O, unnormalised against m
+  float top[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
 
-  // kBatch records' loads go out before any of them is used
-  template <int kBatch, typename At>
+  template <int kBatch, typename At>  // kBatch records' loads go out together
   __device__ void run(int count, int item, int lane, const At& at) {
     const int c = (item % NT) * 8 + 2 * (lane & 3);
     for (int k0 = 0; k0 < count; k0 += kBatch) {
-      float4 v[kBatch];
-      float2 vm[kBatch], vl[kBatch], vs[kBatch];
+      float4 v[kBatch], st[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const bool have = k0 + b < count;
-        const float* rec = at(have ? k0 + b : k0);
-        v[b] = Rec::template get<kGlobal>(rec, item, lane);
-        vm[b] = Rec::template pair<kGlobal>(rec, Rec::kM, c);
-        vl[b] = Rec::template pair<kGlobal>(rec, Rec::kL, c);
-        vs[b] = Rec::template pair<kGlobal>(rec, Rec::kS, c);
+        st[b] = make_float4(kNoMax, 0.f, kNoMax, 0.f);
+        v[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + b < count) {
+          const float* rec = at(k0 + b);
+          st[b] = Rec::template stats<kGlobal>(rec, c);
+          v[b] = Rec::template get<kGlobal>(rec, item, lane);
+        }
       }
+      float t0 = top[0], t1 = top[1];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const float xm[2] = {vm[b].x, vm[b].y}, xl[2] = {vl[b].x, vl[b].y}, xs[2] = {vs[b].x, vs[b].y};
-        const float xo[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
-        if (k0 + b >= count) continue;
+        t0 = fmaxf(t0, st[b].x);
+        t1 = fmaxf(t1, st[b].z);
+      }
+      if (k0 > 0) {
+        const float a0 = fast_exp2(top[0] - t0), a1 = fast_exp2(top[1] - t1);
+        l[0] *= a0;
+        l[1] *= a1;
+        o[0] *= a0;
+        o[1] *= a1;
+        o[2] *= a0;
+        o[3] *= a1;
+      }
+      top[0] = t0;
+      top[1] = t1;
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          const float mn = fmaxf(m[cc], xm[cc]);
-          const float a = fast_exp2(m[cc] - mn), w = fast_exp2(xm[cc] - mn) * xl[cc];
-          m[cc] = mn;
-          l[cc] = l[cc] * a + w;
-          o[cc] = o[cc] * a + xo[cc] * (w * xs[cc]);
-          o[2 + cc] = o[2 + cc] * a + xo[2 + cc] * (w * xs[cc]);
+      for (int b = 0; b < kBatch; ++b) {
+        if (k0 + b < count) {
+          float w0 = fast_exp2(st[b].x - t0), w1 = fast_exp2(st[b].z - t1);
+          if (st[b].x == kNoMax) w0 = 0.f;  // also where every record of the column saw nothing
+          if (st[b].z == kNoMax) w1 = 0.f;
+          l[0] += w0;
+          l[1] += w1;
+          w0 *= st[b].y;
+          w1 *= st[b].w;
+          o[0] = fmaf(v[b].x, w0, o[0]);
+          o[1] = fmaf(v[b].y, w1, o[1]);
+          o[2] = fmaf(v[b].z, w0, o[2]);
+          o[3] = fmaf(v[b].w, w1, o[3]);
         }
       }
     }
@@ -368,6 +397,32 @@ __device__ __forceinline__ uint32_t box_off(int tok, int chunk) {
 __device__ __forceinline__ uint32_t cvt_lo(uint32_t w) { return fp8x2_to_f16x2((uint16_t)w); }
 __device__ __forceinline__ uint32_t cvt_hi(uint32_t w) { return fp8x2_to_f16x2((uint16_t)(w >> 16)); }
 
+// ldmatrix and mma without `volatile`, so that the compiler may overlap one step's loads with
+// another's products. What keeps them in place: their address comes from hold() after the stage's
+// wait, and the products are held before the stage is refilled.
+__device__ __forceinline__ void load_frag(uint32_t addr, uint32_t (&r)[4]) {
+  asm("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void load_frag_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t hold(uint32_t x) {
+  asm volatile("" : "+r"(x) : : "memory");
+  return x;
+}
+__device__ __forceinline__ void hold4(float (&c)[4]) {
+  asm volatile("" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : : "memory");
+}
+
 __device__ __forceinline__ float scale_exp(float s) {  // floor(log2 s), bounded
   return (float)min(127, max(kFp8MinExp, (int)((__float_as_uint(s) >> 23) & 255) - 127));
 }
@@ -380,14 +435,14 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   constexpr int kChunks = D / 16;           // 16-byte chunks of a token row = k-steps of Q K^T
   constexpr int kBox = kSub * D;            // bytes of one box
   constexpr int kStage = 4 * kBox;          // K lo, K hi, V lo, V hi
-  constexpr bool kQShared = NT > 2;         // Q fragments in shared memory
-  constexpr int kQBytes = kQShared ? kChunks * NT * 32 * 8 : 0;
-  using Rec = Fp8Record<D, NT, std::is_same<T, __half>::value && NT <= 2>;  // a warp's
-  using Joined = Fp8Record<D, NT, true>;                                   // a CTA's
+  using Rec = Fp8Record<D, NT, std::is_same<T, __half>::value>;  // a warp's
+  using Joined = Fp8Record<D, NT, true>;                        // a CTA's
   struct Cut {  // a segment that a warp left as a record, in shared memory
     int v, nt;
     int in_ring;  // the stream's last segment: in the warp's ring, done with by then
+    int head;     // the first of its sequence's cuts in this CTA
     int cb;       // first tile of v
+    int row0, col0, cols;
   };
   __shared__ Cut cuts[W][2];
   __shared__ int num_cuts[W];
@@ -401,8 +456,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.y;
   uint8_t* ring = smem + (size_t)warp * S * kStage;
-  uint2* qsm = reinterpret_cast<uint2*>(smem + (size_t)W * S * kStage + (size_t)warp * kQBytes);
-  uint8_t* firsts = smem + (size_t)W * (S * kStage + kQBytes);  // [W][record]: cuts in mid-stream
+  uint8_t* firsts = smem + (size_t)W * S * kStage;  // [W][record]: cuts in mid-stream
   uint64_t* full = reinterpret_cast<uint64_t*>(firsts + (size_t)W * Rec::kFloats * 4) + warp * S;
   static_assert(Rec::kFloats * 4 <= S * kStage && Rec::kFloats % 4 == 0, "a ring holds a record");
   auto record_of = [&](int w, bool in_ring) {
@@ -555,7 +609,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
     }
 
     // ---- Q fragments: column nn * 8 + g8, dims 16c + 4 t4 .. + 3 (8 bytes per lane and k-step)
-    uint2 qf[kQShared ? 1 : kChunks][kQShared ? 1 : NT];
+    uint2 qf[kChunks][NT];
     float qfac[NT][2];  // scale_log2 / (power of two the query row was multiplied by)
 #pragma unroll
     for (int nn = 0; nn < NT; ++nn) {
@@ -592,14 +646,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       // the factor of column 2 t4 + cc sits in the lanes whose g8 is that column
       qfac[nn][0] = __shfl_sync(0xffffffffu, inv, 8 * t4) * p.scale_log2;
       qfac[nn][1] = __shfl_sync(0xffffffffu, inv, 8 * t4 + 4) * p.scale_log2;
-      if constexpr (kQShared) {
-        if (nn == 0) __syncwarp();  // the previous segment's reads are done
 #pragma unroll
-        for (int kk = 0; kk < kChunks; ++kk) qsm[(kk * NT + nn) * 32 + lane] = w[kk];
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < kChunks; ++kk) qf[kk][nn] = w[kk];
-      }
+      for (int kk = 0; kk < kChunks; ++kk) qf[kk][nn] = w[kk];
     }
     // keys that each of this lane's columns sees (columns past the last: none)
     int lim[NT][2];
@@ -663,7 +711,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         }
         __syncwarp();
       }
-      const uint32_t base = smem_u32(stage);
+      const uint32_t base = hold(smem_u32(stage));
 
       // ---- S^T = K Q^T: 2 x 16 tokens, NC columns
       float s[2][NT][4];
@@ -675,22 +723,16 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         const uint32_t mine = base + box_off<D>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
-          uint2 b[2][NT];
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int nn = 0; nn < NT; ++nn)
-              b[j][nn] = kQShared ? qsm[((c + j) * NT + nn) * 32 + lane] : qf[kQShared ? 0 : c + j][kQShared ? 0 : nn];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3;
-            ldmatrix_x4((mine + h * kBox) ^ (uint32_t)(c << 4), a0, a1, a2, a3);
+            uint32_t a[4];
+            load_frag((mine + h * kBox) ^ (uint32_t)(c << 4), a);
 #pragma unroll
             for (int nn = 0; nn < NT; ++nn)
-              MmaOp<__half>::run(s[h][nn], cvt_lo(a0), cvt_lo(a1), cvt_hi(a0), cvt_hi(a1), b[0][nn].x, b[0][nn].y);
+              mma_f16(s[h][nn], cvt_lo(a[0]), cvt_lo(a[1]), cvt_hi(a[0]), cvt_hi(a[1]), qf[c][nn].x, qf[c][nn].y);
 #pragma unroll
             for (int nn = 0; nn < NT; ++nn)
-              MmaOp<__half>::run(s[h][nn], cvt_lo(a2), cvt_lo(a3), cvt_hi(a2), cvt_hi(a3), b[1][nn].x, b[1][nn].y);
+              mma_f16(s[h][nn], cvt_lo(a[2]), cvt_lo(a[3]), cvt_hi(a[2]), cvt_hi(a[3]), qf[c + 1][nn].x, qf[c + 1][nn].y);
           }
         }
       }
@@ -776,19 +818,23 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         for (int c = 0; c < kChunks; c += 2) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3;
-            ldmatrix_x4_trans((mine + h * kBox) ^ (uint32_t)(c << 4), a0, a1, a2, a3);
-            a0 = __byte_perm(a0, 0, 0x3120), a1 = __byte_perm(a1, 0, 0x3120);
-            a2 = __byte_perm(a2, 0, 0x3120), a3 = __byte_perm(a3, 0, 0x3120);
+            uint32_t a[4];
+            load_frag_trans((mine + h * kBox) ^ (uint32_t)(c << 4), a);
+#pragma unroll
+            for (int k2 = 0; k2 < 4; ++k2) a[k2] = __byte_perm(a[k2], 0, 0x3120);
 #pragma unroll
             for (int nn = 0; nn < NT; ++nn)
-              MmaOp<__half>::run(acc[c][nn], cvt_lo(a0), cvt_hi(a0), cvt_lo(a1), cvt_hi(a1), pb[h][nn][0], pb[h][nn][1]);
+              mma_f16(acc[c][nn], cvt_lo(a[0]), cvt_hi(a[0]), cvt_lo(a[1]), cvt_hi(a[1]), pb[h][nn][0], pb[h][nn][1]);
 #pragma unroll
             for (int nn = 0; nn < NT; ++nn)
-              MmaOp<__half>::run(acc[c + 1][nn], cvt_lo(a2), cvt_hi(a2), cvt_lo(a3), cvt_hi(a3), pb[h][nn][0], pb[h][nn][1]);
+              mma_f16(acc[c + 1][nn], cvt_lo(a[2]), cvt_hi(a[2]), cvt_lo(a[3]), cvt_hi(a[3]), pb[h][nn][0], pb[h][nn][1]);
           }
         }
       }
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+        for (int nn = 0; nn < NT; ++nn) hold4(acc[i][nn]);
       // Refill the stage: its reads fed the MMAs above; generic writes need a proxy fence before
       // the TMA unit writes the same bytes.
       if (valid < kTile) fence_proxy_async_smem();
@@ -835,14 +881,12 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         if (g8 == 0) {
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
-            rec[Rec::kM + nn * 8 + 2 * t4 + cc] = mx[nn][cc];
-            rec[Rec::kL + nn * 8 + 2 * t4 + cc] = l[nn][cc];
-            rec[Rec::kS + nn * 8 + 2 * t4 + cc] =
-                l[nn][cc] > 0.f ? top[cc] * (fast_exp2(my[nn][cc] - mx[nn][cc]) / l[nn][cc]) : 0.f;
+            Rec::put_stats(rec, nn * 8 + 2 * t4 + cc, weight_of(mx[nn][cc], l[nn][cc]),
+                           l[nn][cc] > 0.f ? top[cc] * (fast_exp2(my[nn][cc] - mx[nn][cc]) / l[nn][cc]) : 0.f);
           }
         }
       }
-      if (lane == 0 && ncut < 2) cuts[warp][ncut] = Cut{v, ntl, in_ring, cb};
+      if (lane == 0 && ncut < 2) cuts[warp][ncut] = Cut{v, ntl, in_ring, lb0 == 0 || warp == 0, cb, t.row0, t.col0, t.cols};
       ++ncut;
     }
     gidx = seg_end;
@@ -859,99 +903,103 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
     }
 
   // ---- merge what this CTA's warps left. The cuts, in tile order, fall into groups of one
-  // virtual sequence each; all warps walk the groups together.
+  // virtual sequence each: a head cut and the first cut of each further warp up to the sequence's
+  // end. Lane e looks at cut e % 2 of warp e / 2; a piece of work is one fragment (item) of a group.
   if (lane == 0) num_cuts[warp] = ncut;
   __syncthreads();
+  constexpr int kItems = kChunks * NT;
+  static_assert(2 * W <= 32, "a lane per cut");
   const int cta_unit = blockIdx.x * W;
   const int cta_begin = r.start(cta_unit), cta_end = r.start(min(cta_unit + W, r.parts));
-  auto write_item = [&](int v, int item, const float (&o)[4], const float (&l)[2]) {
-    const Virtual t = virtual_of<NC>(p, v);
+  Cut mine{};
+  int u_end = 0;       // unit that holds the end of the lane's sequence
+  bool open = false, closed = false;
+  if (lane < 2 * W && (lane & 1) < num_cuts[lane >> 1]) {
+    mine = cuts[lane >> 1][lane & 1];
+    u_end = r.unit_of(mine.cb + mine.nt - 1);
+    const bool inside = mine.cb >= cta_begin && mine.cb + mine.nt <= cta_end;
+    open = mine.head && !inside;  // other CTAs hold a part of the sequence
+    closed = mine.head && inside;
+  }
+  const unsigned opens = __ballot_sync(0xffffffffu, open), closeds = __ballot_sync(0xffffffffu, closed);
+  // rows of the output from one merged fragment
+  auto write_item = [&](int row0, int col0, int cols, int item, const float (&o)[4], const float (&l)[2]) {
     const int i = item / NT, nn = item % NT;
 #pragma unroll
     for (int cc = 0; cc < 2; ++cc) {
       const int c = nn * 8 + 2 * t4 + cc;
-      if (c >= t.cols) continue;
-      const int col = t.col0 + c;
+      if (c >= cols) continue;
+      const int row = row_of(p, col0 + c);
       const float f = l[cc] > 0.f ? 1.f / l[cc] : 0.f;
-      T* orow = reinterpret_cast<T*>(p.out) + (int64_t)(t.row0 + row_of(p, col)) * p.o_tok +
-                (int64_t)(head * p.group + col - row_of(p, col) * p.group) * p.o_head;
+      T* orow = reinterpret_cast<T*>(p.out) + (int64_t)(row0 + row) * p.o_tok +
+                (int64_t)(head * p.group + col0 + c - row * p.group) * p.o_head;
       *reinterpret_cast<uint32_t*>(orow + i * 16 + 2 * g8) = pack2<T>(o[cc] * f, o[2 + cc] * f);
     }
   };
-  constexpr int kItems = kChunks * NT;
-  int open_v[2], open_cb[2], open_c0[2], open_c1[2];  // sequences that CTAs c0 .. c1 share
-  int opens = 0;
-  for (int w = 0, c = 0;;) {
-    while (w < W && c >= num_cuts[w]) ++w, c = 0;
-    if (w == W) break;
-    const Cut g = cuts[w][c];
-    // the group: this cut and the first one of each further warp up to the sequence's end
-    const int u1 = r.unit_of(g.cb + g.nt - 1);
-    const int w1 = min(W - 1, u1 - cta_unit);
-    const bool whole = g.cb >= cta_begin && g.cb + g.nt <= cta_end;
-    float* joined = p.joined + (((size_t)head * gridDim.x + blockIdx.x) * 2 + (g.cb <= cta_begin ? 0 : 1)) * Joined::kFloats;
-    for (int item = warp; item < kItems; item += W) {
+  // The warp's share of the pieces of the groups in `heads`.
+  auto merge_groups = [&](unsigned heads, bool inside) {
+    const int pieces = __popc(heads) * kItems;
+    const int per = (pieces + W - 1) / W;
+    const int end = min(pieces, (warp + 1) * per);
+    for (int piece = warp * per; piece < end; ++piece) {
+      unsigned m = heads;
+      for (int skip = piece / kItems; skip > 0; --skip) m &= m - 1;
+      const int item = piece % kItems, e = __ffs(m) - 1, w0 = e >> 1;
+      const int w1 = min(W - 1, __shfl_sync(0xffffffffu, u_end, e) - cta_unit);
+      // a warp between the first and the last of a group has one segment, its stream's last
+      const int ring0 = __shfl_sync(0xffffffffu, mine.in_ring, e);
+      const int ring1 = __shfl_sync(0xffffffffu, mine.in_ring, 2 * w1);
+      const int cb = __shfl_sync(0xffffffffu, mine.cb, e);
+      const int row0 = __shfl_sync(0xffffffffu, mine.row0, e);
+      const int col0 = __shfl_sync(0xffffffffu, mine.col0, e), cols = __shfl_sync(0xffffffffu, mine.cols, e);
       Merge<Rec, NT, false> mg;
-      mg.template run<2>(w1 - w + 1, item, lane, [&](int k) -> const float* {
-        return record_of(w + k, (k == 0 ? g : cuts[w + k][0]).in_ring);
+      mg.template run<4>(w1 - w0 + 1, item, lane, [&](int k) -> const float* {
+        return record_of(w0 + k, k == 0 ? ring0 : k == w1 - w0 ? ring1 : 1);
       });
-      if (whole) {
-        write_item(g.v, item, mg.o, mg.l);
+      if (inside) {
+        write_item(row0, col0, cols, item, mg.o, mg.l);
         continue;
       }
+      float* joined = p.joined + (((size_t)head * gridDim.x + blockIdx.x) * 2 + (cb <= cta_begin ? 0 : 1)) * Joined::kFloats;
       const float i0 = mg.l[0] > 0.f ? 1.f / mg.l[0] : 0.f, i1 = mg.l[1] > 0.f ? 1.f / mg.l[1] : 0.f;
       Joined::put(joined, item, lane, mg.o[0] * i0, mg.o[1] * i1, mg.o[2] * i0, mg.o[3] * i1);
       if (item < NT && g8 == 0) {
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-          joined[Joined::kM + item * 8 + 2 * t4 + cc] = mg.m[cc];
-          joined[Joined::kL + item * 8 + 2 * t4 + cc] = mg.l[cc];
-          joined[Joined::kS + item * 8 + 2 * t4 + cc] = 1.f;
+          Joined::put_stats(joined, item * 8 + 2 * t4 + cc, weight_of(mg.top[cc], mg.l[cc]), 1.f);
         }
       }
     }
-    if (!whole && opens < 2) {
-      open_v[opens] = g.v;
-      open_cb[opens] = g.cb;
-      open_c0[opens] = r.unit_of(g.cb) / W;
-      open_c1[opens] = u1 / W;
-      ++opens;
-    }
-    if (w1 == w) {
-      ++c;
-    } else {
-      w = w1;
-      c = 1;
+  };
+  // The open groups (at most two) first: their counts travel while the closed ones are written.
+  if (opens != 0) {
+    merge_groups(opens, false);
+    __syncthreads();  // the CTA's joined records are written
+    if (warp == 0 && open) {
+      int seen;
+      int32_t* counter = p.counters + (size_t)head * nv + mine.v;
+      asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(counter) : "memory");
+      const bool last = seen == u_end / W - r.unit_of(mine.cb) / W;
+      if (last) *counter = 0;  // for the next launch
+      last_of[mine.cb <= cta_begin ? 0 : 1] = last;
     }
   }
-  if (opens == 0) return;  // the same for the whole CTA
-  __syncthreads();  // the CTA's joined records are written
-  if (threadIdx.x == 0) {
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");
-    int seen[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)  // both in flight together
-      seen[j] = j < opens ? atomicAdd(p.counters + (size_t)head * nv + open_v[j], 1) : -1;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (j >= opens) continue;
-      const bool is_last = seen[j] == open_c1[j] - open_c0[j];
-      last_of[j] = is_last;
-      if (is_last) p.counters[(size_t)head * nv + open_v[j]] = 0;  // for the next launch
-    }
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");
-  }
+  if (closeds != 0) merge_groups(closeds, true);
+  if (opens == 0) return;
   __syncthreads();
-  for (int j = 0; j < opens; ++j) {
-    if (!last_of[j]) continue;
+  for (unsigned m = opens; m != 0; m &= m - 1) {
+    const int e = __ffs(m) - 1;
+    const int cb = __shfl_sync(0xffffffffu, mine.cb, e);
+    if (!last_of[cb <= cta_begin ? 0 : 1]) continue;
+    const int c0 = r.unit_of(cb) / W, c1 = __shfl_sync(0xffffffffu, u_end, e) / W;
+    const int row0 = __shfl_sync(0xffffffffu, mine.row0, e);
+    const int col0 = __shfl_sync(0xffffffffu, mine.col0, e), cols = __shfl_sync(0xffffffffu, mine.cols, e);
     for (int item = warp; item < kItems; item += W) {
       Merge<Joined, NT, true> mg;
-      mg.template run<4>(open_c1[j] - open_c0[j] + 1, item, lane, [&](int k) -> const float* {
-        const int c = open_c0[j] + k;
-        const int slot = open_cb[j] <= r.start(c * W) ? 0 : 1;
-        return p.joined + (((size_t)head * gridDim.x + c) * 2 + slot) * Joined::kFloats;
+      mg.template run<8>(c1 - c0 + 1, item, lane, [&](int k) -> const float* {
+        return p.joined + (((size_t)head * gridDim.x + c0 + k) * 2 + (cb <= r.start((c0 + k) * W) ? 0 : 1)) * Joined::kFloats;
       });
-      write_item(open_v[j], item, mg.o, mg.l);
+      write_item(row0, col0, cols, item, mg.o, mg.l);
     }
   }
 }
@@ -964,13 +1012,13 @@ struct Fp8Plan {
 
 template <typename T, int D, int NT, int S, int W>
 Fp8Plan make_fp8_plan() {
-  static_assert(NT <= 4 && D <= 128, "the workspace has room for these");
+  static_assert(NT <= 2 && D <= 128, "the workspace has room for these");
   Fp8Plan pl;
   pl.fn = reinterpret_cast<const void*>(&paged_rows_fp8<T, D, NT, S, W>);
-  using Rec = Fp8Record<D, NT, std::is_same<T, __half>::value && NT <= 2>;
-  pl.smem = W * S * 4 * kSub * D + (NT > 2 ? W * (D / 16) * NT * 32 * 8 : 0) + W * Rec::kFloats * 4 + W * S * 8 + 1024;
-  static_assert(W * S * 4 * kSub * D + (NT > 2 ? W * (D / 16) * NT * 32 * 8 : 0) + W * Rec::kFloats * 4 + W * S * 8 +
-                        1024 + W * 64 + 64 <= 227 * 1024, "shared memory of an SM");
+  using Rec = Fp8Record<D, NT, std::is_same<T, __half>::value>;
+  pl.smem = W * S * 4 * kSub * D + W * Rec::kFloats * 4 + W * S * 8 + 1024;
+  static_assert(W * S * 4 * kSub * D + W * Rec::kFloats * 4 + W * S * 8 + 1024 + W * 100 + 64 <= 227 * 1024,
+                "shared memory of an SM");
   pl.warps = W;
   pl.columns = NT * 8;
   return pl;
@@ -979,13 +1027,9 @@ Fp8Plan make_fp8_plan() {
 template <typename T>
 bool select_fp8_plan(int head_dim, int columns, Fp8Plan& pl) {
   if (head_dim == 128)
-    pl = columns <= 8 ? make_fp8_plan<T, 128, 1, 2, 8>()
-         : columns <= 16 ? make_fp8_plan<T, 128, 2, 2, 8>()
-                         : make_fp8_plan<T, 128, 4, 2, 6>();
+    pl = columns <= 8 ? make_fp8_plan<T, 128, 1, 2, 8>() : make_fp8_plan<T, 128, 2, 2, 8>();
   else if (head_dim == 64)
-    pl = columns <= 8 ? make_fp8_plan<T, 64, 1, 4, 8>()
-         : columns <= 16 ? make_fp8_plan<T, 64, 2, 4, 8>()
-                         : make_fp8_plan<T, 64, 4, 4, 8>();
+    pl = columns <= 8 ? make_fp8_plan<T, 64, 1, 4, 8>() : make_fp8_plan<T, 64, 2, 4, 8>();
   else
     return false;
   return true;
@@ -1001,7 +1045,7 @@ int64_t fp8_ctas(int num_kv_heads) {
 // sit at one place for every shape and call, in bytes that nothing else ever writes. (At a place
 // that followed the call's own records, one buffer used for calls of one and of five rows in
 // turn would find records where it looks for zeroed counters.)
-constexpr int kMostColumns = 32;   // per virtual sequence
+constexpr int kMostColumns = 16;   // per virtual sequence
 constexpr int kRowColumns = 64;    // columns per sequence that calls here have at most
 
 size_t records_bytes(int num_kv_heads) {
@@ -1019,7 +1063,7 @@ int column_groups(const Fp8Plan& pl, int group, int max_q_len) {
 bool b2p_rows_fp8_takes(int group, int head_dim, int block_size, int dtype, int max_q_len) {
   Fp8Plan pl;
   return (dtype == B2P_BF16 || dtype == B2P_F16) && block_size % kSub == 0 && max_q_len >= 1 &&
-         (max_q_len > 1 || group <= 32) && (int64_t)group * max_q_len <= kRowColumns &&
+         (int64_t)group * max_q_len <= kRowColumns &&
          select_fp8_plan<__half>(head_dim, group * max_q_len, pl);
 }
 
