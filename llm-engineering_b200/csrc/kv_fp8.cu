@@ -8,7 +8,9 @@
 // sequence touches only the first can hold older rows; where the new rows need a larger
 // scale there, the older codes are rounded to it in the same pass.
 //   e_new = max(e_old if the write leaves the block's first slot alone, e(amax of the new rows))
-// The work is pure streaming: every new row is read once, its codes are written once.
+// The work is pure streaming: every new row is read once, its codes are written once. A warp holds
+// its rows in registers between the two (16 rows of 128 take 8 16-byte pieces a lane); where they
+// do not fit it reads them again, from L2.
 #include "fp8.cuh"
 
 namespace {
@@ -29,46 +31,161 @@ struct WriteFp8Params {
   const int32_t* ctx;
   int64_t num_rows, num_blocks;
   int num_seqs, max_q_len, touched, hkv, d, block_size;
+  bool vec;  // every row of keys and values starts on a 16-byte boundary
   int32_t* err;
 };
 
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-  return x;
-}
-
-// One warp: the rows [row0, row0 + n) of one head into slots off0 .. off0 + n - 1 of a block.
+// Eight elements of a row: values, and the running maximum of their magnitudes as bits (magnitudes
+// of floats are ordered as their bits are; infinities and NaN come out on top).
 template <typename T>
-__device__ void write_block_head(const T* src, int64_t tok, uint8_t* dst, int64_t row_bytes,
-                                 float* scale, int d, int off0, int n, int lane) {
-  float amax = 0.f;
-  bool bad = false;
-  for (int i = lane; i < n * d; i += 32) {
-    const float x = to_f32<T>(src[(int64_t)(i / d) * tok + i % d]);
-    bad |= fp8_bad(x);
-    amax = fmaxf(amax, fabsf(x));
+struct Piece {  // bf16, f16
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void max_bits(uint32_t& m) const {
+    m = __vmaxu2(m, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
   }
-  amax = warp_max(amax);
-  bad = __any_sync(0xffffffffu, bad);
-  float old = 0.f;
-  if (off0 > 0) old = *scale;  // one address: every lane sees the same value
-  __syncwarp();
-  bad |= off0 > 0 && !(old <= 3.402823466e38f);
-  const float s = bad ? 1.f : fmaxf(exp2_int(fp8_block_exp(fminf(amax, kFp8Saturate))), old);
-  if (off0 > 0 && !bad && s != old) {
-    const float shift = old / s;  // a power of two, at most 1/2
-    for (int i = lane; i < off0 * d; i += 32) {
-      uint8_t* c = dst + (int64_t)(i / d) * row_bytes + i % d;
-      *c = fp8_code(fp8_value(*c), shift);
+  __device__ static __forceinline__ float magnitude(uint32_t m) {
+    const uint16_t b = (uint16_t)max(m & 0xffffu, m >> 16);
+    return to_f32<T>(*reinterpret_cast<const T*>(&b));
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t b = (uint16_t)(in[i >> 1] >> (16 * (i & 1)));
+      x[i] = to_f32<T>(*reinterpret_cast<const T*>(&b));
     }
   }
-  const float inv = 1.f / s;
+};
+
+template <>
+struct Piece<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const float4*>(p));
+    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ void max_bits(uint32_t& m) const {
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  }
+  __device__ static __forceinline__ float magnitude(uint32_t m) { return __uint_as_float(m); }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+};
+
+// Four codes of x * inv, ties to even.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+  const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | (uint32_t)hi << 16;
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const Piece<T>& p, float inv, bool clamp) {
+  float x[8];
+  p.values(x);
+  if (clamp) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -kFp8Saturate), kFp8Saturate);
+  }
+  return make_uint2(codes4(x[0], x[1], x[2], x[3], inv), codes4(x[4], x[5], x[6], x[7], inv));
+}
+
+// The block's scale from the largest magnitude of its new rows; NaN where a row is not finite or
+// the scale it keeps already is. `old` counts where the write leaves the block's first slot alone.
+__device__ __forceinline__ float new_scale(float amax, float old, bool keep) {
+  const bool bad = !(amax <= 3.402823466e38f) || (keep && !(old <= 3.402823466e38f));
+  if (bad) return __int_as_float(0x7fffffff);
+  const float s = exp2_int(fp8_block_exp(fminf(amax, kFp8Saturate)));
+  return keep ? fmaxf(s, old) : s;
+}
+
+// The codes of the block's older rows, rounded to the larger scale.
+__device__ __forceinline__ void rescale(uint8_t* dst, int64_t row_bytes, int d, int rows, float shift, int lane) {
+  const int per_row = d / 8;
+  for (int i = lane; i < rows * per_row; i += 32) {
+    uint2* at = reinterpret_cast<uint2*>(dst + (int64_t)(i / per_row) * row_bytes) + i % per_row;
+    const uint2 w = *at;
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = fp8_value((uint8_t)((k < 4 ? w.x : w.y) >> (8 * (k & 3))));
+    *at = make_uint2(codes4(x[0], x[1], x[2], x[3], shift), codes4(x[4], x[5], x[6], x[7], shift));
+  }
+}
+
+constexpr int kHold = 8;  // pieces of eight elements that a lane keeps
+
+// One warp: n rows of one head into slots off0 .. off0 + n - 1 of a block, by 16-byte pieces.
+template <typename T>
+__device__ void write_block_vec(const T* src, int64_t tok, uint8_t* dst, int64_t row_bytes,
+                                float* scale, int d, int off0, int n, int lane) {
+  const int per_row = d / 8, total = n * per_row;
+  const bool keep = off0 > 0;
+  const float old = keep ? *scale : 0.f;  // one address for the warp
+  uint32_t m = 0;
+  Piece<T> held[kHold];
+  const bool fits = total <= 32 * kHold;
+  auto at = [&](int i) { return src + (int64_t)(i / per_row) * tok + (i % per_row) * 8; };
+  if (fits) {
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      if (lane + 32 * k < total) held[k].load(at(lane + 32 * k));
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      if (lane + 32 * k < total) held[k].max_bits(m);
+  } else {
+    for (int i = lane; i < total; i += 32) {
+      held[0].load(at(i));
+      held[0].max_bits(m);
+    }
+  }
+  const float amax = Piece<T>::magnitude(m);
+  // bits again: __reduce_max_sync orders NaN and infinities above every number
+  const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+  const float s = new_scale(top, old, keep);
+  const bool bad = s != s;
+  if (keep && !bad && s != old) rescale(dst, row_bytes, d, off0, old / s, lane);
+  const float inv = bad ? 0.f : 1.f / s;
+  const bool clamp = top > kFp8Saturate;
+  auto put = [&](int i, const Piece<T>& p) {
+    const uint2 c = bad ? make_uint2(0u, 0u) : codes8<T>(p, inv, clamp);
+    reinterpret_cast<uint2*>(dst + (int64_t)(off0 + i / per_row) * row_bytes)[i % per_row] = c;
+  };
+  if (fits) {
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      if (lane + 32 * k < total) put(lane + 32 * k, held[k]);
+  } else {
+    for (int i = lane; i < total; i += 32) {
+      held[0].load(at(i));
+      put(i, held[0]);
+    }
+  }
+  if (lane == 0) *scale = s;
+}
+
+// The same by single elements, for rows that are not 16-byte aligned.
+template <typename T>
+__device__ void write_block_elem(const T* src, int64_t tok, uint8_t* dst, int64_t row_bytes,
+                                 float* scale, int d, int off0, int n, int lane) {
+  const bool keep = off0 > 0;
+  const float old = keep ? *scale : 0.f;
+  uint32_t m = 0;
+  for (int i = lane; i < n * d; i += 32)
+    m = max(m, __float_as_uint(to_f32<T>(src[(int64_t)(i / d) * tok + i % d])) & 0x7fffffffu);
+  const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+  const float s = new_scale(top, old, keep);
+  const bool bad = s != s;
+  if (keep && !bad && s != old) rescale(dst, row_bytes, d, off0, old / s, lane);
+  const float inv = bad ? 0.f : 1.f / s;
   for (int i = lane; i < n * d; i += 32) {
     const float x = to_f32<T>(src[(int64_t)(i / d) * tok + i % d]);
     dst[(int64_t)(off0 + i / d) * row_bytes + i % d] = bad ? 0 : fp8_code(x, inv);
   }
-  if (lane == 0) *scale = bad ? __int_as_float(0x7fffffff) : s;
+  if (lane == 0) *scale = s;
 }
 
 template <typename T>
@@ -104,8 +221,11 @@ __global__ void __launch_bounds__(128) kv_write_fp8_rows(const WriteFp8Params p)
     const int64_t row = q0 + (lo - start);
     const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) +
                    (is_v ? row * p.v_tok + h * p.v_head : row * p.k_tok + h * p.k_head);
-    write_block_head<T>(src, is_v ? p.v_tok : p.k_tok, dst, row_bytes, scale, p.d,
-                        lo - b * p.block_size, hi - lo, lane);
+    const int off0 = lo - b * p.block_size;
+    if (p.vec)
+      write_block_vec<T>(src, is_v ? p.v_tok : p.k_tok, dst, row_bytes, scale, p.d, off0, hi - lo, lane);
+    else
+      write_block_elem<T>(src, is_v ? p.v_tok : p.k_tok, dst, row_bytes, scale, p.d, off0, hi - lo, lane);
   }
 }
 
@@ -122,31 +242,49 @@ struct ReadFp8Params {
   int32_t* err;
 };
 
-// One thread per 8 codes of a row (head_dim is a multiple of 8).
+// One thread per 8 codes of a row (head_dim is a multiple of 8); the pieces of two rounds are in
+// flight together.
 template <typename T>
-__global__ void __launch_bounds__(256) kv_read_fp8(const ReadFp8Params p) {
-  const int64_t per_row = (int64_t)p.hkv * p.d / 8;
+__global__ void __launch_bounds__(256) kv_read_fp8_rows(const ReadFp8Params p) {
+  const int per_row = p.hkv * p.d / 8, per_head = p.d / 8;
   const int64_t total = p.num_rows * per_row * 2;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / (per_row * 2);
-    const int64_t rem = i - row * per_row * 2;
-    const bool is_v = rem >= per_row;
-    const int c = (int)(is_v ? rem - per_row : rem);
-    const int32_t slot = __ldg(p.slots + row);
-    T* out = reinterpret_cast<T*>(is_v ? p.v : p.k) + row * per_row * 8 + c * 8;
-    if (slot >= p.num_slots && c == 0 && !is_v) set_device_error(p.err, B2P_DEV_SLOT_RANGE);
-    const bool have = slot >= 0 && slot < p.num_slots;
-    uint2 raw = make_uint2(0u, 0u);
-    float s = 0.f;
-    if (have) {
-      raw = __ldg(reinterpret_cast<const uint2*>((is_v ? p.v_cache : p.k_cache) + slot * per_row * 8) + c);
-      s = __ldg((is_v ? p.v_scales : p.k_scales) + (int64_t)(slot / p.block_size) * p.hkv + c * 8 / p.d);
+  const int64_t step = gridDim.x * 256ll;
+  for (int64_t i0 = blockIdx.x * 256ll + threadIdx.x; i0 < total; i0 += 2 * step) {
+    uint2 raw[2];
+    float s[2];
+    T* out[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t i = i0 + k * step;
+      out[k] = nullptr;
+      raw[k] = make_uint2(0u, 0u);
+      s[k] = 0.f;
+      if (i >= total) continue;
+      const int64_t row = i / (2 * per_row);
+      const int rem = (int)(i - row * 2 * per_row);
+      const bool is_v = rem >= per_row;
+      const int c = is_v ? rem - per_row : rem;
+      out[k] = reinterpret_cast<T*>(is_v ? p.v : p.k) + (row * per_row + c) * 8;
+      const int32_t slot = __ldg(p.slots + row);
+      if (slot >= p.num_slots && rem == 0) set_device_error(p.err, B2P_DEV_SLOT_RANGE);
+      if (slot < 0 || slot >= p.num_slots) continue;
+      raw[k] = __ldg(reinterpret_cast<const uint2*>(is_v ? p.v_cache : p.k_cache) + (int64_t)slot * per_row + c);
+      s[k] = __ldg((is_v ? p.v_scales : p.k_scales) + (int64_t)(slot / p.block_size) * p.hkv + c / per_head);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint8_t code = (uint8_t)((e < 4 ? raw.x : raw.y) >> (8 * (e & 3)));
-      out[e] = from_f32<T>(fp8_value(code) * s);
+    for (int k = 0; k < 2; ++k) {
+      if (out[k] == nullptr) continue;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = fp8_value((uint8_t)((e < 4 ? raw[k].x : raw[k].y) >> (8 * (e & 3)))) * s[k];
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(out[k])[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(out[k])[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
+        *reinterpret_cast<uint4*>(out[k]) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
+                                                       pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+      }
     }
   }
 }
@@ -177,6 +315,8 @@ extern "C" int b2p_kv_write_fp8(const void* keys, int64_t k_tok_stride, int64_t 
   if (!keys || !values || !key_cache || !value_cache || !key_scales || !value_scales ||
       !block_tables || !cu_seqlens_q || !context_lens)
     return B2P_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 7u)
+    return B2P_EINVAL;
   WriteFp8Params p;
   p.k = static_cast<const uint8_t*>(keys);
   p.v = static_cast<const uint8_t*>(values);
@@ -202,6 +342,9 @@ extern "C" int b2p_kv_write_fp8(const void* keys, int64_t k_tok_stride, int64_t 
   p.d = head_dim;
   p.block_size = block_size;
   p.err = err_flag;
+  const int es = element_size(dtype);
+  p.vec = ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values) | (uintptr_t)(k_tok_stride * es) |
+            (uintptr_t)(k_head_stride * es) | (uintptr_t)(v_tok_stride * es) | (uintptr_t)(v_head_stride * es)) & 15u) == 0;
   const int64_t warps = (int64_t)num_seqs * p.touched * num_kv_heads * 2;
   const int64_t most = (int64_t)b2p_host::sm_count() * 16;
   const unsigned grid = (unsigned)((warps + 3) / 4 < most ? (warps + 3) / 4 : most);
@@ -230,7 +373,8 @@ extern "C" int b2p_kv_read_fp8(const void* key_cache, const void* value_cache,
   if (num_rows == 0) return B2P_OK;
   if (!key_cache || !value_cache || !key_scales || !value_scales || !slot_mapping || !keys || !values)
     return B2P_EINVAL;
-  if ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 7u)
+  if (((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 7u) ||
+      ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15u))
     return B2P_EINVAL;
   ReadFp8Params p;
   const int64_t row = (int64_t)num_kv_heads * head_dim;
@@ -253,10 +397,10 @@ extern "C" int b2p_kv_read_fp8(const void* key_cache, const void* value_cache,
   const unsigned grid = (unsigned)((items + 255) / 256 < most ? (items + 255) / 256 : most);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == B2P_BF16)
-    kv_read_fp8<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+    kv_read_fp8_rows<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
   else if (dtype == B2P_F16)
-    kv_read_fp8<__half><<<grid, 256, 0, s>>>(p);
+    kv_read_fp8_rows<__half><<<grid, 256, 0, s>>>(p);
   else
-    kv_read_fp8<float><<<grid, 256, 0, s>>>(p);
+    kv_read_fp8_rows<float><<<grid, 256, 0, s>>>(p);
   return b2p_host::check_launch();
 }

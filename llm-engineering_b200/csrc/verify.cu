@@ -10,12 +10,14 @@
 // stream this gives is distributed as the target model's own.
 //
 // Bytes: a handful of gathered values, then one row pair (p_n, q_n) per sequence, read once;
-// everything else is latency. One cluster of kCluster CTAs owns a sequence: every CTA takes a
-// slice of the vocabulary and every warp a contiguous piece of the slice; the piece sums meet
-// in distributed shared memory, and only the one piece that holds the crossing is read again
+// everything else is latency. One cluster of CTAs owns a sequence: every CTA takes a slice of the
+// vocabulary and every warp a contiguous piece of the slice, in 16-byte loads; the piece sums
+// meet in distributed shared memory, and only the one piece that holds the crossing is read again
 // (from L2) to find the index. All sums are fp64 in a fixed order: p - q and u * q of fp32
 // inputs are exact there, and a token's interval is as narrow as its probability, so fp32
-// sums over 150,000 entries would move draws across the borders of rare tokens.
+// sums over 150,000 entries would move draws across the borders of rare tokens. (The
+// conversions to fp64, two per entry, are what an SM has least of: a quarter of the time that
+// the entry's 8 bytes take from HBM.)
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -28,7 +30,7 @@ using namespace b2p;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCluster = 8;
+constexpr int kMostRanks = 8;  // CTAs of a cluster
 
 struct VerifyParams {
   const uint8_t* target;  // [total + num_seqs, vocab]
@@ -50,13 +52,13 @@ struct VerifyParams {
 // What a CTA needs to know of its sequence.
 struct Row {
   int begin, k, n;   // first draft, drafts, accepted
-  int64_t rejected;  // the rejected token, -1: none (or out of range)
+  int rejected;      // the rejected token, -1: none (or out of range)
 };
 
 __device__ __forceinline__ double positive(double x) { return x > 0.0 ? x : 0.0; }  // NaN: 0
 
 template <typename T>
-__device__ __forceinline__ double residual(const T* p, const T* q, int64_t drop, int v) {
+__device__ __forceinline__ double residual(const T* p, const T* q, int drop, int v) {
   const double x = (double)to_f32<T>(p[v]);
   if (q != nullptr) return positive(x - (double)to_f32<T>(q[v]));
   return v == drop ? 0.0 : positive(x);
@@ -68,12 +70,59 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
+// Sum of the residual over [v0, v1) of one warp's piece, in 16-byte loads where both rows start on
+// a 16-byte boundary (pieces do within a row).
+template <typename T, bool kDraft>
+__device__ __forceinline__ double piece_sum(const T* p, const T* q, int drop, int v0, int v1, int lane) {
+  constexpr int kPer = 16 / sizeof(T);
+  double s = 0.0;
+  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0) {
+    constexpr int kAhead = 4;  // loads of each row in flight per lane
+    const int whole = v0 + (v1 - v0) / kPer * kPer;  // the row's last piece may end unaligned
+    for (int v = v0 + lane * kPer; v < whole; v += 32 * kPer * kAhead) {
+      uint4 a[kAhead], b[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int at = v + k * 32 * kPer;
+        a[k] = b[k] = make_uint4(0, 0, 0, 0);
+        if (at < whole) {
+          a[k] = __ldcs(reinterpret_cast<const uint4*>(p + at));
+          if (kDraft) b[k] = __ldcs(reinterpret_cast<const uint4*>(q + at));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const T* x = reinterpret_cast<const T*>(&a[k]);
+        const T* y = reinterpret_cast<const T*>(&b[k]);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          float u = to_f32<T>(x[e]);
+          if (kDraft) {
+            float w = to_f32<T>(y[e]);
+            const bool more = u > w;  // false for NaN
+            u = more ? u : 0.f;
+            w = more ? w : 0.f;
+            s += (double)u - (double)w;
+          } else {
+            s += (double)(u > 0.f && v + k * 32 * kPer + e != drop ? u : 0.f);
+          }
+        }
+      }
+    }
+    if (whole + lane < v1) s += residual<T>(p, kDraft ? q : nullptr, drop, whole + lane);
+  } else {
+    for (int v = v0 + lane; v < v1; v += 32) s += residual<T>(p, kDraft ? q : nullptr, drop, v);
+  }
+  return warp_sum(s);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_drafts(const VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 2) verify_drafts(const VerifyParams p) {
   __shared__ Row row;
-  __shared__ double piece[2][kWarps];  // [residual, target][warp]: sums over the warp's piece
-  __shared__ double totals[2];         // this CTA's
-  __shared__ int pick;
+  __shared__ double piece[kWarps];  // sums over the warps' pieces
+  __shared__ double total;          // this CTA's
+  __shared__ double scan[kWarps];
+  __shared__ int pick, tail;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank();
   const int ranks = (int)cluster.num_blocks();
@@ -111,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) verify_drafts(const VerifyParams p) 
       if (stop) {
         const int first = __ffs(stop) - 1;
         r.n = base + first;
-        r.rejected = __shfl_sync(0xffffffffu, x, first);
+        r.rejected = (int)__shfl_sync(0xffffffffu, x, first);
         break;
       }
       r.n = min(base + 32, r.k);
@@ -124,7 +173,10 @@ __global__ void __launch_bounds__(kThreads) verify_drafts(const VerifyParams p) 
       if (lane == 0) p.accepted[seq] = r.n;
     }
   }
-  if (threadIdx.x == 0) pick = p.vocab;
+  if (threadIdx.x == 0) {
+    pick = p.vocab;
+    tail = -1;
+  }
   __syncthreads();
   if (row.k < 0) return;  // the whole cluster returns
 
@@ -133,49 +185,45 @@ __global__ void __launch_bounds__(kThreads) verify_drafts(const VerifyParams p) 
   const T* qrow = rejected && p.draft != nullptr
                       ? reinterpret_cast<const T*>(p.draft) + (int64_t)(row.begin + row.n) * p.d_row
                       : nullptr;
-  const int64_t drop = rejected && p.draft == nullptr ? row.rejected : -1;
-  // the vocabulary in ranks * kWarps pieces, in index order
-  const int len = (p.vocab + ranks * kWarps - 1) / (ranks * kWarps);
+  int drop = rejected && p.draft == nullptr ? row.rejected : -1;
+  // the vocabulary in ranks * kWarps pieces, in index order, each a multiple of 16 bytes
+  constexpr int kPer = 16 / sizeof(T);
+  const int len = ((p.vocab + ranks * kWarps - 1) / (ranks * kWarps) + kPer - 1) / kPer * kPer;
   const int v0 = min(p.vocab, (rank * kWarps + warp) * len), v1 = min(p.vocab, v0 + len);
-  double r = 0.0, t = 0.0;
-#pragma unroll 4
-  for (int v = v0 + lane; v < v1; v += 32) {
-    r += residual<T>(prow, qrow, drop, v);
-    t += positive((double)to_f32<T>(prow[v]));
-  }
-  r = warp_sum(r);
-  t = warp_sum(t);
-  if (lane == 0) {
-    piece[0][warp] = r;
-    piece[1][warp] = t;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double s = 0.0;
-    for (int w = 0; w < kWarps; ++w) s += piece[threadIdx.x][w];
-    totals[threadIdx.x] = s;
-  }
-  cluster.sync();
-  double all[2] = {0.0, 0.0}, before[2] = {0.0, 0.0};
-  double part[2][kCluster];
-  for (int c = 0; c < kCluster; ++c) {
-    for (int k = 0; k < 2; ++k) {
-      part[k][c] = c < ranks ? *cluster.map_shared_rank(&totals[k], c) : 0.0;
-      if (c == rank) before[k] = all[k];
-      all[k] += part[k][c];
+  double part[kMostRanks];
+  double all = 0.0;
+  for (int pass = 0; pass < 2; ++pass) {
+    const double s = qrow != nullptr ? piece_sum<T, true>(prow, qrow, -1, v0, v1, lane)
+                                     : piece_sum<T, false>(prow, nullptr, drop, v0, v1, lane);
+    if (lane == 0) piece[warp] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double t = 0.0;
+      for (int w = 0; w < kWarps; ++w) t += piece[w];
+      total = t;
     }
+    cluster.sync();
+    all = 0.0;
+#pragma unroll
+    for (int c = 0; c < kMostRanks; ++c) {
+      part[c] = c < ranks ? *cluster.map_shared_rank(&total, c) : 0.0;
+      all += part[c];
+    }
+    cluster.sync();  // nobody leaves or writes again while its total may still be read
+    if (all > 0.0 || (qrow == nullptr && drop < 0)) break;
+    qrow = nullptr;  // nothing left over (p <= q everywhere): the target row itself
+    drop = -1;
   }
-  cluster.sync();  // nobody leaves while its totals may still be read
-  // nothing left over (p <= q everywhere): the target row itself
-  const int use = all[0] > 0.0 ? 0 : 1;
-  const double goal = (double)p.sample[seq] * all[use];
+  const double goal = (double)p.sample[seq] * all;
   // the CTA that holds the crossing; where rounding or a draw outside [0, 1) leaves none, the
   // last one with anything in it
   int owner = -1, last = -1;
-  double run = 0.0;
-  for (int c = 0; c < ranks; ++c) {
-    run += part[use][c];
-    if (part[use][c] > 0.0) {
+  double run = 0.0, base = 0.0;
+#pragma unroll
+  for (int c = 0; c < kMostRanks; ++c) {
+    if (c == rank) base = run;
+    run += part[c];
+    if (part[c] > 0.0) {
       last = c;
       if (owner < 0 && run > goal) owner = c;
     }
@@ -188,10 +236,10 @@ __global__ void __launch_bounds__(kThreads) verify_drafts(const VerifyParams p) 
   if (owner != rank) return;
   // the same inside the CTA, over its warps' pieces
   int ow = -1, lw = -1;
-  double base = before[use], start = base;
+  double start = base;
   for (int w = 0; w < kWarps; ++w) {
-    const double next = base + piece[use][w];
-    if (piece[use][w] > 0.0) {
+    const double next = base + piece[w];
+    if (piece[w] > 0.0) {
       lw = w;
       if (ow < 0) start = base;
       if (ow < 0 && next > goal) ow = w;
@@ -204,26 +252,21 @@ __global__ void __launch_bounds__(kThreads) verify_drafts(const VerifyParams p) 
   const int w0 = min(p.vocab, (rank * kWarps + ow) * len), w1 = min(p.vocab, w0 + len);
   const int per = (len + kThreads - 1) / kThreads;
   const int a = min(w1, w0 + (int)threadIdx.x * per), b = min(w1, a + per);
-  const T* qr = use == 0 ? qrow : nullptr;
-  const int64_t dr = use == 0 ? drop : -1;
   double mine = 0.0;
-  for (int v = a; v < b; ++v) mine += residual<T>(prow, qr, dr, v);
+  for (int v = a; v < b; ++v) mine += residual<T>(prow, qrow, drop, v);
   double incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double y = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += y;
   }
-  __shared__ double scan[kWarps];
-  __shared__ int tail;
-  if (threadIdx.x == 0) tail = -1;
   if (lane == 31) scan[warp] = incl;
   __syncthreads();
   double at = start;
   for (int w = 0; w < warp; ++w) at += scan[w];
   at += incl - mine;
   for (int v = a; v < b; ++v) {
-    const double x = residual<T>(prow, qr, dr, v);
+    const double x = residual<T>(prow, qrow, drop, v);
     at += x;
     if (x > 0.0) {
       atomicMax(&tail, v);
@@ -305,12 +348,17 @@ extern "C" int b2p_verify_drafts(const void* target_probs, int64_t target_row_st
   p.accepted = out_accepted;
   p.err = err_flag;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)num_seqs * kCluster);
+  // CTAs per sequence: as many as fill the GPU with one wave (two CTAs per SM). More only repeat
+  // the search for the first rejected draft: 256 sequences over 151,936 entries take 48.7 us with
+  // one CTA each, 52 with two, 76 with eight; one sequence takes 23.6, 15.4 and 8.8 us.
+  int ranks = kMostRanks;
+  while (ranks > 1 && (int64_t)num_seqs * ranks > 2LL * b2p_host::sm_count()) ranks /= 2;
+  cfg.gridDim = dim3((unsigned)(num_seqs * ranks));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.x = ranks;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
