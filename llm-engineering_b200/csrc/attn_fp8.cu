@@ -78,52 +78,83 @@ struct WidenParams {
   int32_t* err;
 };
 
-// code * scale in T; f16 keeps its largest finite value where the product passes it.
+// f16 keeps its largest finite value where a product passes it.
 template <typename T>
-__device__ __forceinline__ T widen(uint8_t code, float s) {
-  float x = fp8_value(code) * s;
-  if (std::is_same<T, __half>::value) x = x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
-  return from_f32<T>(x);
+__device__ __forceinline__ float bounded(float x) {
+  return std::is_same<T, __half>::value ? (x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x) : x;
 }
 
-// One CTA per (sequence, block): its codes as 16-bit rows in the scratch block that the scratch
-// table gives it. Memory-bound: 1 byte read and 2 written per element.
+// A CTA takes the used blocks of all histories in turn (found by a scan of the lengths, 32
+// sequences at a time: with one CTA per table entry, most of a ragged batch's are empty, 35 us
+// against 17 on 32 prompts) and writes their codes as 16-bit rows into the scratch block that the
+// scratch table gives them. Memory-bound: 1 byte read and 2 written per element.
 template <typename T>
 __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenParams p) {
-  const int64_t total = (int64_t)p.num_seqs * p.width;
-  for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-    const int seq = (int)(w / p.width), col = (int)(w - (int64_t)seq * p.width);
-    const int ctx = __ldg(p.ctx + seq);
-    const int q0 = __ldg(p.cu + seq), q1 = __ldg(p.cu + seq + 1);
-    if (threadIdx.x == 0) p.tables[w] = (int32_t)w;
-    if (q1 <= q0) continue;  // no row reads this history
-    if (col == 0) {
-      // rows before the first position see nothing: zeros (the tile kernel may skip them)
-      const int blind = min(q1 - q0, q1 - q0 - max(ctx, 0));
-      if (blind > 0 && threadIdx.x == 0) set_device_error(p.err, B2P_DEV_LENGTH);
-      if (ctx > (int64_t)p.width * p.block_size && threadIdx.x == 0)
-        set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
-      for (int64_t e = threadIdx.x; e < (int64_t)max(blind, 0) * p.hq * p.d; e += kWidenThreads) {
-        const int64_t row = q0 + e / (p.hq * p.d);
-        const int r = (int)(e % (p.hq * p.d));
-        if (row >= 0 && row < p.num_rows)
-          reinterpret_cast<T*>(p.out)[row * p.o_tok + (int64_t)(r / p.d) * p.o_head + r % p.d] = from_f32<T>(0.f);
+  __shared__ int found[2];  // sequence (-1: no block left) and block number
+  const int lane = threadIdx.x & 31;
+  // rows before a sequence's first position see nothing: zeros (the tile kernel may skip them)
+  for (int seq = blockIdx.x; seq < p.num_seqs; seq += gridDim.x) {
+    const int q0 = __ldg(p.cu + seq), rows = __ldg(p.cu + seq + 1) - q0, ctx = __ldg(p.ctx + seq);
+    const int blind = min(rows, rows - max(ctx, 0));
+    if (threadIdx.x == 0 && rows > 0) {
+      if (blind > 0) set_device_error(p.err, B2P_DEV_LENGTH);
+      if (ctx > (int64_t)p.width * p.block_size) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
+    }
+    for (int64_t e = threadIdx.x; e < (int64_t)max(blind, 0) * p.hq * p.d; e += kWidenThreads) {
+      const int64_t row = q0 + e / (p.hq * p.d);
+      const int r = (int)(e % (p.hq * p.d));
+      if (row >= 0 && row < p.num_rows)
+        reinterpret_cast<T*>(p.out)[row * p.o_tok + (int64_t)(r / p.d) * p.o_head + r % p.d] = from_f32<T>(0.f);
+    }
+  }
+  for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
+    __syncthreads();  // the previous round has read `found`
+    if (threadIdx.x < 32) {
+      int64_t want = unit;
+      int seq = -1, col = 0;
+      for (int base = 0; base < p.num_seqs && seq < 0; base += 32) {
+        const int s = base + lane;
+        int n = 0;
+        if (s < p.num_seqs && __ldg(p.cu + s + 1) > __ldg(p.cu + s))
+          n = min(p.width, (max(__ldg(p.ctx + s), 0) + p.block_size - 1) / p.block_size);
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, incl > want);
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          seq = base + src;
+          col = (int)(want - __shfl_sync(0xffffffffu, incl - n, src));
+        } else {
+          want -= __shfl_sync(0xffffffffu, incl, 31);
+        }
+      }
+      if (lane == 0) {
+        found[0] = seq;
+        found[1] = col;
       }
     }
-    const int tokens = min(p.block_size, ctx - col * p.block_size);
-    if (tokens <= 0) continue;
+    __syncthreads();
+    const int seq = found[0], col = found[1];
+    if (seq < 0) return;
+    const int64_t w = (int64_t)seq * p.width + col;
+    if (threadIdx.x == 0) p.tables[w] = (int32_t)w;
+    const int tokens = min(p.block_size, __ldg(p.ctx + seq) - col * p.block_size);
     const int32_t blk = __ldg(p.block_tables + (int64_t)seq * p.bt_stride + col);
     const bool have = blk >= 0 && blk < p.num_blocks;
     if (!have && threadIdx.x == 0) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
-    const int per_row = p.hkv * p.d / 16;  // 16-code pieces
+    const int per_row = p.hkv * p.d / 16, per_head = p.d / 16;  // 16-code pieces
     for (int i = threadIdx.x; i < 2 * tokens * per_row; i += kWidenThreads) {
       const bool is_v = i >= tokens * per_row;
-      const int64_t at = is_v ? i - tokens * per_row : i;
+      const int at = is_v ? i - tokens * per_row : i;
       uint4 raw = make_uint4(0, 0, 0, 0);
       float s = 0.f;
       if (have) {
         raw = __ldg(reinterpret_cast<const uint4*>(p.codes[is_v]) + (int64_t)blk * p.block_size * per_row + at);
-        const int64_t sc = (int64_t)blk * p.hkv + (int)(at % per_row) * 16 / p.d;
+        const int64_t sc = (int64_t)blk * p.hkv + at % per_row / per_head;
         const float sk = __ldg(p.scales[0] + sc), sv = __ldg(p.scales[1] + sc);
         // A NaN value block shows through the scores alone: rows that do not see it would
         // otherwise meet it as 0 * NaN in P V.
@@ -133,10 +164,9 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
       const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const uint16_t two = (uint16_t)(in[k >> 1] >> (16 * (k & 1)));
-        const T lo = widen<T>((uint8_t)two, s), hi = widen<T>((uint8_t)(two >> 8), s);
-        words[k] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) |
-                   (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+        const uint32_t two = fp8x2_to_f16x2((uint16_t)(in[k >> 1] >> (16 * (k & 1))));
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&two));
+        words[k] = pack2<T>(bounded<T>(x.x * s), bounded<T>(x.y * s));
       }
       uint4* to = reinterpret_cast<uint4*>(p.wide[is_v]) + (w * p.block_size * per_row + at) * 2;
       to[0] = make_uint4(words[0], words[1], words[2], words[3]);

@@ -121,34 +121,29 @@ __device__ int scan_cta(int x, int* shared, int& total) {
 __global__ void __launch_bounds__(kPlanThreads) plan_moves(const CompactPlan pl, int64_t num_blocks,
                                                            int32_t* new_ids, int32_t* num_live) {
   __shared__ int shared[kPlanThreads / 32];
-  const int64_t words = (num_blocks + 31) / 32;
-  const int64_t per = (words + kPlanThreads - 1) / kPlanThreads;
-  const int64_t w0 = min(words, (int64_t)threadIdx.x * per), w1 = min(words, w0 + per);
-  int mine = 0, live = 0;
-  for (int64_t w = w0; w < w1; ++w) mine += __popc(pl.bits[w]);
+  const int64_t per = (num_blocks + kPlanThreads - 1) / kPlanThreads;
+  const int64_t b0 = min(num_blocks, (int64_t)threadIdx.x * per), b1 = min(num_blocks, b0 + per);
+  auto live_at = [&](int64_t b) { return (int)((pl.bits[b >> 5] >> (b & 31)) & 1u); };
+  int mine = 0, live = 0, moves = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += live_at(b);
   scan_cta(mine, shared, live);
-  // blocks of word w that lie below / at and past num_live
-  auto below = [&](int64_t w) -> uint32_t {
-    const int64_t n = live - w * 32;
-    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-  };
-  int holes = 0, movers = 0, moves = 0;
-  for (int64_t w = w0; w < w1; ++w) {
-    holes += __popc(~pl.bits[w] & below(w));
-    movers += __popc(pl.bits[w] & ~below(w));
+  int holes = 0, movers = 0;
+  for (int64_t b = b0; b < b1; ++b) {
+    const int is_live = live_at(b);
+    holes += b < live && !is_live;
+    movers += b >= live && is_live;
   }
   int h = scan_cta(holes, shared, moves);
   int m = scan_cta(movers, shared, moves);
-  for (int64_t w = w0; w < w1; ++w) {
-    for (uint32_t x = ~pl.bits[w] & below(w); x; x &= x - 1) pl.dst[h++] = (int32_t)(w * 32 + __ffs(x) - 1);
-    for (uint32_t x = pl.bits[w] & ~below(w); x; x &= x - 1) pl.src[m++] = (int32_t)(w * 32 + __ffs(x) - 1);
+  for (int64_t b = b0; b < b1; ++b) {
+    const int is_live = live_at(b);
+    if (b < live && !is_live) pl.dst[h++] = (int32_t)b;
+    if (b >= live && is_live) pl.src[m++] = (int32_t)b;
   }
   __syncthreads();  // the targets of all threads are written
   m -= movers;
-  for (int64_t b = w0 * 32; b < min(num_blocks, w1 * 32); ++b) {
-    const bool is_live = (pl.bits[b >> 5] >> (b & 31)) & 1;
-    new_ids[b] = !is_live ? -1 : b < live ? (int32_t)b : pl.dst[m++];
-  }
+  for (int64_t b = b0; b < b1; ++b)
+    new_ids[b] = !live_at(b) ? -1 : b < live ? (int32_t)b : pl.dst[m++];
   if (threadIdx.x == 0) {
     *pl.moves = moves;
     *num_live = live;
