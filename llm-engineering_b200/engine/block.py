@@ -2,13 +2,14 @@
 
 Allocation order is part of the contract, because slot mappings must match the
 reference bit for bit: free blocks leave from the head of a FIFO queue and a block
-whose last reference is released rejoins at its tail.
+whose last reference is released rejoins at its tail. Forks (shared full blocks) and
+compaction are additions, which nothing in the reference's policy uses.
 """
 
 from __future__ import annotations
 
 from collections import deque
-from collections.abc import Iterable
+from collections.abc import Iterable, Sequence
 from dataclasses import dataclass
 
 
@@ -81,6 +82,23 @@ class BlockPool:
         for b in block_ids:
             self.free(b)
 
+    def apply_moves(self, new_ids: Sequence[int]) -> None:
+        """Adopt a compaction: block b is now block new_ids[b] (-1: b is free). Reference counts
+        move with the blocks; the free queue restarts in ascending order."""
+        if len(new_ids) != self.num_blocks:
+            raise ValueError("new_ids must have one entry per block.")
+        refs = [0] * self.num_blocks
+        for old, new in enumerate(new_ids):
+            if (new >= 0) != (self._refs[old] > 0):
+                raise ValueError(f"new_ids and the reference counts disagree on block {old}.")
+            if new >= 0:
+                self._check(new)
+                if refs[new]:
+                    raise ValueError(f"Two blocks move to block {new}.")
+                refs[new] = self._refs[old]
+        self._refs = refs
+        self._free = deque(b for b in range(self.num_blocks) if refs[b] == 0)
+
     def _check(self, block_id: int) -> None:
         if block_id < 0 or block_id >= self.num_blocks:
             raise ValueError(f"Invalid block_id: {block_id!r}.")
@@ -111,6 +129,36 @@ class BlockTable:
     def free_request(self, request_id: str) -> None:
         self.pool.free_many(self._table(request_id))
         del self._tables[request_id]
+
+    def fork_request(self, parent_id: str, child_id: str,
+                     num_tokens: int) -> tuple[tuple[int, int], ...]:
+        """Give child_id the first num_tokens tokens of parent_id. Full blocks are shared (their
+        reference counts grow); a partly filled last block gets a block of its own, because
+        both requests go on writing there. Returns the (source, target) block copies that the
+        cache needs before the child runs (``PagedKVStorage.copy_blocks``): none or one."""
+        parent = self._table(parent_id)
+        if child_id in self._tables:
+            raise ValueError(f"request_id {child_id!r} already has a block table.")
+        if num_tokens <= 0:
+            raise ValueError("num_tokens must be greater than zero.")
+        full, rest = divmod(num_tokens, self.block_size)
+        if full + (rest > 0) > len(parent):
+            raise ValueError("num_tokens is more than the parent's blocks hold.")
+        own = list(self.pool.allocate(1)) if rest else []
+        for b in parent[:full]:
+            self.pool.increment_ref_count(b)
+        self._tables[child_id] = parent[:full] + own
+        return tuple((parent[full], b) for b in own)
+
+    def tables(self) -> dict[str, tuple[int, ...]]:
+        """Every request's blocks."""
+        return {rid: tuple(t) for rid, t in self._tables.items()}
+
+    def apply_moves(self, new_ids: Sequence[int]) -> None:
+        """Adopt a compaction of the pool (``BlockPool.apply_moves``) in every table."""
+        self.pool.apply_moves(new_ids)
+        for table in self._tables.values():
+            table[:] = [new_ids[b] for b in table]
 
     def append_token(self, request_id: str, token_position: int) -> None:
         table = self._table(request_id)

@@ -80,6 +80,10 @@ class StepBatch:
     # Decode rows take the fused K1 + K2 call: the cache hook then writes only the
     # prefill rows, and the attention function stores the decode rows' new K/V itself.
     fused_decode: bool = False
+    # Scales of an 8-bit pool (None: a pool in the model's dtype). Its rows are all appended by
+    # the cache hook, since a block's scale depends on every row in it.
+    key_scales: torch.Tensor | None = None
+    value_scales: torch.Tensor | None = None
 
 
 def _phase_of(execution) -> str:
@@ -112,6 +116,17 @@ def paged_attention(module: torch.nn.Module, query: torch.Tensor, key: torch.Ten
     k = batch.kernels
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     nd = batch.num_decode
+    if batch.key_scales is not None:
+        pool = (batch.key_cache, batch.value_cache, batch.key_scales, batch.value_scales, layer)
+        if nd:
+            k.paged_decode_fp8(q[:nd], *pool, batch.block_tables[:nd], batch.context_lens[:nd],
+                               batch.block_size, scaling, out=out[:nd],
+                               workspace=batch.workspace, err_flag=batch.err)
+        if nd < batch.num_execs:
+            k.paged_prefill_fp8(q, *pool, batch.block_tables[nd:], batch.cu_seqlens_q[nd:],
+                                batch.context_lens[nd:], batch.max_q_len, batch.block_size,
+                                scaling, out=out, workspace=batch.workspace, err_flag=batch.err)
+        return out.unsqueeze(0), None
     if nd and batch.fused_decode:
         k.paged_decode_append(q[:nd], key[0].transpose(0, 1)[:nd], value[0].transpose(0, 1)[:nd],
                               batch.key_cache, batch.value_cache, layer, batch.block_tables[:nd],
@@ -159,6 +174,12 @@ class B200PagedCache(Cache):
                 "Packed KV query length does not match BatchLayout: "
                 f"expected {self._batch.total_q}, got {key_states.shape[2]}.")
         b = self._batch
+        if b.key_scales is not None:
+            b.kernels.kv_write_fp8(b.key_cache, b.value_cache, b.key_scales, b.value_scales,
+                                   layer_idx, b.block_tables, b.cu_seqlens_q, b.context_lens,
+                                   b.max_q_len, b.block_size, key_states[0].transpose(0, 1),
+                                   value_states[0].transpose(0, 1), b.err)
+            return key_states, value_states
         first = b.num_decode if b.fused_decode else 0  # decode rows: stored by the fused call
         if first < b.total_q:
             b.kernels.kv_write(b.key_cache, b.value_cache, layer_idx, b.slot_mapping[first:],
@@ -252,7 +273,8 @@ class B200PagedModelRunner:
         device: CUDA device of the model and the pool.
         paged_cache: the reference's ``PagedKVCache`` (or anything with ``.storage``) or a
             storage object exposing ``key_cache``, ``value_cache`` and ``block_size``
-            (the reference's ``PagedKVStorage`` or ``llm_engineering_b200.storage``).
+            (the reference's ``PagedKVStorage`` or ``llm_engineering_b200.storage``; with
+            ``Fp8PagedKVStorage`` every step appends to and attends over the 8-bit pool).
 
     Every ``forward`` reads the kernels' device error word once the step's logits are
     computed (one synchronisation, which the caller's sampling would make anyway) and
@@ -385,8 +407,14 @@ class B200PagedModelRunner:
         else:
             tables = dev_i32[3 * n:].view(n, width)
             md = kernels.build_metadata(qlens, ctx, rows, tables, bs, total_q, 0, self._err)
-        need = kernels.decode_workspace_size(max(num_decode, 1), self._hq, self._hkv,
-                                             self._head_dim)
+        key_scales = getattr(self._storage, "key_scales", None)
+        if key_scales is not None:
+            if d["block_size"] != self._storage.block_size:
+                raise ValueError("an 8-bit cache needs block-structured slot_ids")
+            need = kernels.fp8_workspace_size(n, self._hq, self._hkv, self._head_dim)
+        else:
+            need = kernels.decode_workspace_size(max(num_decode, 1), self._hq, self._hkv,
+                                                 self._head_dim)
         if self._workspace.numel() < need:
             self._workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
         batch = StepBatch(
@@ -396,7 +424,9 @@ class B200PagedModelRunner:
             slot_mapping=md["slot_mapping"], positions=md["positions"],
             cu_seqlens_q=md["cu_seqlens_q"], context_lens=ctx, block_tables=tables,
             logit_indices=md["logit_indices"], workspace=self._workspace, err=self._err,
-            fused_decode=num_decode > 0 and hasattr(kernels, "paged_decode_append"))
+            fused_decode=(key_scales is None and num_decode > 0
+                          and hasattr(kernels, "paged_decode_append")),
+            key_scales=key_scales, value_scales=getattr(self._storage, "value_scales", None))
         return batch, input_ids
 
     # ------------------------------------------------------------------ ModelRunner
@@ -481,6 +511,11 @@ class B200PagedModelRunner:
                 "kernels take); expect a large slowdown", RuntimeWarning, stacklevel=3)
         return out
 
+    def forget_tables(self) -> None:
+        """Drop the device copy of the block tables (it only learns of new blocks, not of moved
+        ones): call it after ``PagedKVStorage.compact``; the next step uploads whole tables."""
+        self._mirror = None
+
     @staticmethod
     def _fallbacks() -> tuple[int, int] | None:
         """bf16/f16 launches that took the CUDA-core kernels so far (decode, prefill)."""
@@ -507,7 +542,8 @@ class B200PagedModelRunner:
 
 
 _ERROR_BITS = ((1, "slot id outside the pool"), (2, "block id outside the pool"),
-               (4, "a bounded wait gave up"), (8, "a length that does not fit"))
+               (4, "a bounded wait gave up"), (8, "a length that does not fit"),
+               (16, "a drafted token outside the vocabulary"))
 
 
 def _error_names(bits: int) -> list[str]:
