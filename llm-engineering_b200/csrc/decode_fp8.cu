@@ -45,7 +45,7 @@ using namespace b2p;
 
 constexpr int kSub = 16;   // tokens per TMA box (any block size that is a multiple of 16)
 constexpr int kTile = 32;  // tokens per stage
-constexpr float kNoMax = -1e30f;     // reference before the first key (finite: no inf - inf)
+constexpr float kNoMax = -1e30f;     // log2 weight of a record that saw nothing
 constexpr float kSlack = 8.0f;       // log2 units a score may pass its reference by
 constexpr int kL2Prefetch = 4;       // tiles per warp prefetched into L2 before the launch wait
 
@@ -449,9 +449,10 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
   __shared__ int last_of[2];  // per open group: this CTA was the last to count in
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // Programmatic dependent launch, as in the 16-bit decode kernel: before the wait only
-  // lengths, offsets and block tables are read, which no kernel that lets its successor start
-  // early writes (the cache write and the table kernels do not).
+  // Programmatic dependent launch: before the wait only lengths, offsets and block tables are
+  // read. Of the kernels that let this one start early (itself, the 16-bit decode kernel, the
+  // cache write) none writes those, and the kernels that do write them (table builds, compaction,
+  // host copies) have completed before any of these started.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.y;
@@ -525,21 +526,37 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       }
     }
   }
+  // From here on what the previous kernel wrote is read from L2 (TMA, ld.cg): this grid may have
+  // started before those writes, so nothing may come from an L1 line or the read-only path.
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // scales of this lane's tile, by half: loaded with the slots, a chunk ahead of their use
-  float ks_cur[2], vs_cur[2], ks_nxt[2], vs_nxt[2];
-  auto load_scales = [&](const Slots& s, float (&ks)[2], float (&vs)[2]) {
+  // Scales of this lane's tile, by half: loaded with the slots, a chunk ahead of their use. A NaN
+  // value scale moves to the key scale: the scores then carry it to the rows that see the block,
+  // and to no others.
+  struct Scales {
+    float k[2], v[2], e[2];  // e: floor(log2 v), bounded
+  };
+  auto load_scales = [&](const Slots& s, Scales& c) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bool have = s.block[h] >= 0;
       const int64_t at = (int64_t)(have ? s.block[h] : 0) * p.hkv + head;
-      ks[h] = have ? __ldg(p.k_scales + at) : 0.f;
-      vs[h] = have ? __ldg(p.v_scales + at) : 0.f;
+      c.k[h] = have ? __ldcg(p.k_scales + at) : 0.f;
+      c.v[h] = have ? __ldcg(p.v_scales + at) : 0.f;
     }
   };
-  load_scales(cur, ks_cur, vs_cur);
-  ks_nxt[0] = ks_nxt[1] = vs_nxt[0] = vs_nxt[1] = 0.f;
+  auto settle_scales = [](Scales& c) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (c.v[h] != c.v[h]) {
+        c.k[h] = c.v[h];
+        c.v[h] = 0.f;
+      }
+      c.e[h] = scale_exp(c.v[h]);
+    }
+  };
+  Scales sc_cur, sc_nxt{};
+  load_scales(cur, sc_cur);
   int issue_base = 0;  // tiles [issue_base, issue_base + 32) are in the issue slots
   Slots isl = cur;     // slots that the issue side reads (may run a chunk ahead of the scales)
   int issued = 0, use_base = 0, issue_stage = 0;
@@ -621,7 +638,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       uint2 w[kChunks];
 #pragma unroll
       for (int kk = 0; kk < kChunks; ++kk)
-        w[kk] = ok ? __ldg(reinterpret_cast<const uint2*>(qrow + kk * 16)) : make_uint2(0u, 0u);
+        w[kk] = ok ? __ldcg(reinterpret_cast<const uint2*>(qrow + kk * 16)) : make_uint2(0u, 0u);
       float inv = 1.f;
       if constexpr (!std::is_same<T, __half>::value) {
         float amax = 0.f;
@@ -661,11 +678,12 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       }
     if (p.cu != nullptr) lim_min = t.ctx - t.qlen + row_of(p, t.col0) + 1;
 
-    float mx[NT][2], my[NT][2], gy[NT][2], l[NT][2];
+    float mx[NT][2], slack[NT][2], gy[NT][2], l[NT][2];
     float acc[kChunks][NT][4];
 #pragma unroll
     for (int nn = 0; nn < NT; ++nn) {
-      mx[nn][0] = mx[nn][1] = my[nn][0] = my[nn][1] = kNoMax;
+      mx[nn][0] = mx[nn][1] = 0.f;  // set by the segment's first tile
+      slack[nn][0] = slack[nn][1] = kSlack;
       gy[nn][0] = gy[nn][1] = 1.f;
       l[nn][0] = l[nn][1] = 0.f;
     }
@@ -677,18 +695,20 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
     for (int lb = lb0; lb < lb1; ++lb, ++k) {
       if (k == use_base + 32) {  // rotate the scale buffers; the issue side has moved on already
         use_base += 32;
-        ks_cur[0] = ks_nxt[0], ks_cur[1] = ks_nxt[1], vs_cur[0] = vs_nxt[0], vs_cur[1] = vs_nxt[1];
+        sc_cur = sc_nxt;
       }
       if (k == use_base + 8 && use_base + 32 < n) {  // the next chunk, well before it is issued
         nxt = res(p, nv, use_base + 32, lane, num_slots);
-        load_scales(nxt, ks_nxt, vs_nxt);
+        load_scales(nxt, sc_nxt);
       }
+      if (k == use_base) settle_scales(sc_cur);
       const int src = k - use_base;
-      float ks[2], vs[2];
+      float ks[2], vs[2], ev[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ks[h] = __shfl_sync(0xffffffffu, ks_cur[h], src);
-        vs[h] = __shfl_sync(0xffffffffu, vs_cur[h], src);
+        ks[h] = __shfl_sync(0xffffffffu, sc_cur.k[h], src);
+        vs[h] = __shfl_sync(0xffffffffu, sc_cur.v[h], src);
+        ev[h] = __shfl_sync(0xffffffffu, sc_cur.e[h], src);
       }
       if (!aborted && !mbar_wait_bounded(full + use_stage, phase, p.err)) aborted = true;
       aborted = __any_sync(0xffffffffu, aborted);
@@ -737,18 +757,20 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         }
       }
 
-      // ---- scores in log2 units, masked where a column's rows end
+      // ---- scores in log2 units less m_x, masked where a column's rows end. A score may pass
+      // its references by kSlack: thr is what is left of that for m_x and, with the half's
+      // exponent, for m_y (slack = m_y - m_x + kSlack).
       const bool masked = tok0 + kTile > lim_min;
-      bool over = false;
-      const float ev[2] = {scale_exp(vs[0]), scale_exp(vs[1])};
+      const bool first = lb == lb0;
+      bool over = first;
 #pragma unroll
       for (int nn = 0; nn < NT; ++nn)
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          const float f = qfac[nn][cc];
+        for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float x0 = s[h][nn][cc] * (ks[h] * f), x1 = s[h][nn][2 + cc] * (ks[h] * f);
+            const float f = ks[h] * qfac[nn][cc];
+            float x0 = fmaf(s[h][nn][cc], f, -mx[nn][cc]), x1 = fmaf(s[h][nn][2 + cc], f, -mx[nn][cc]);
             if (masked) {
               const int left = lim[nn][cc] - tok0 - h * kSub;
               if (g8 >= left) x0 = -INFINITY;
@@ -756,10 +778,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
             }
             s[h][nn][cc] = x0;
             s[h][nn][2 + cc] = x1;
-            const float top = fmaxf(x0, x1);
-            over |= top - mx[nn][cc] > kSlack || top + ev[h] - my[nn][cc] > kSlack;
+            over |= fmaxf(x0, x1) > fminf(kSlack, slack[nn][cc] - ev[h]);
           }
-        }
       if (__any_sync(0xffffffffu, over)) {  // move the references (always on a segment's first tile)
 #pragma unroll
         for (int nn = 0; nn < NT; ++nn)
@@ -771,18 +791,33 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
               t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
               t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
             }
-            const float nx = fmaxf(mx[nn][cc], fmaxf(t0, t1));
-            const float ny = fmaxf(my[nn][cc], fmaxf(t0 + ev[0], t1 + ev[1]));
-            l[nn][cc] *= fast_exp2(mx[nn][cc] - nx);
-            const float al = fast_exp2(my[nn][cc] - ny);
+            // By how much m_x and m_y move (t0, t1 are relative to m_x): to the first tile's
+            // largest, later only up. A column that sees nothing of the first tile sees nothing of
+            // the later ones either (its keys end before them).
+            const float gap = slack[nn][cc] - kSlack;  // m_y - m_x
+            float dx = fmaxf(t0, t1), dy = fmaxf(t0 + ev[0], t1 + ev[1]) - gap;
+            if (first) {
+              dx = dx == -INFINITY ? 0.f : dx;
+              dy = dy == -INFINITY ? 0.f : dy;
+            } else {
+              dx = fmaxf(dx, 0.f);
+              dy = fmaxf(dy, 0.f);
+              l[nn][cc] *= fast_exp2(-dx);
+              const float al = fast_exp2(-dy);
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i) {
-              acc[i][nn][cc] *= al;
-              acc[i][nn][2 + cc] *= al;
+              for (int i = 0; i < kChunks; ++i) {
+                acc[i][nn][cc] *= al;
+                acc[i][nn][2 + cc] *= al;
+              }
             }
-            mx[nn][cc] = nx;
-            my[nn][cc] = ny;
-            gy[nn][cc] = fast_exp2(nx - ny);
+            mx[nn][cc] += dx;
+            slack[nn][cc] += dy - dx;
+            gy[nn][cc] = fast_exp2(kSlack - slack[nn][cc]);  // 2^(m_x - m_y)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[h][nn][cc] -= dx;
+              s[h][nn][2 + cc] -= dx;
+            }
           }
       }
       // ---- P = 2^(x - m_x); its f16 copy carries vs against m_y
@@ -794,17 +829,12 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
           float pv[4];
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
-            const float p0 = fast_exp2(s[h][nn][cc] - mx[nn][cc]), p1 = fast_exp2(s[h][nn][2 + cc] - mx[nn][cc]);
+            const float p0 = fast_exp2(s[h][nn][cc]), p1 = fast_exp2(s[h][nn][2 + cc]);
             l[nn][cc] += p0 + p1;
-            float f = vs[h] * gy[nn][cc];
-            f = f > 0x1p126f ? 0x1p126f : f;  // a block whose weights have all underflowed; NaN stays
+            // bounded: a block whose weights have all underflowed may have any factor
+            const float f = fminf(vs[h] * gy[nn][cc], 0x1p126f);
             pv[cc] = p0 * f;
             pv[2 + cc] = p1 * f;
-            if (masked) {  // 0 * NaN of a poisoned block
-              const int left = lim[nn][cc] - tok0 - h * kSub;
-              if (g8 >= left) pv[cc] = 0.f;
-              if (g8 + 8 >= left) pv[2 + cc] = 0.f;
-            }
           }
           pb[h][nn][0] = movmatrix_trans(pack2<__half>(pv[0], pv[1]));
           pb[h][nn][1] = movmatrix_trans(pack2<__half>(pv[2], pv[3]));
@@ -856,7 +886,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       for (int nn = 0; nn < NT; ++nn)
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc)
-          f[nn][cc] = l[nn][cc] > 0.f ? fast_exp2(my[nn][cc] - mx[nn][cc]) / l[nn][cc] : 0.f;
+          f[nn][cc] = l[nn][cc] > 0.f ? fast_exp2(slack[nn][cc] - kSlack) / l[nn][cc] : 0.f;
       write_out(t, acc, f);
     } else {
       const bool in_ring = seg_end == r.end;
@@ -882,7 +912,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
             Rec::put_stats(rec, nn * 8 + 2 * t4 + cc, weight_of(mx[nn][cc], l[nn][cc]),
-                           l[nn][cc] > 0.f ? top[cc] * (fast_exp2(my[nn][cc] - mx[nn][cc]) / l[nn][cc]) : 0.f);
+                           l[nn][cc] > 0.f ? top[cc] * (fast_exp2(slack[nn][cc] - kSlack) / l[nn][cc]) : 0.f);
           }
         }
       }

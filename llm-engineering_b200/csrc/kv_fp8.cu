@@ -212,6 +212,9 @@ __device__ __forceinline__ int touched_blocks(const Append& a, int block_size) {
 // A unit is (sequence, touched block, head, K or V), one per warp and round.
 template <typename T>
 __global__ void __launch_bounds__(128) kv_write_fp8_rows(const WriteFp8Params p) {
+  // The attention that follows may start its look at lengths and tables, which this kernel does
+  // not write, while it runs; it waits for this grid's end before it touches the pool.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int per_block = 2 * p.hkv;
   const int64_t per_seq = (int64_t)p.touched * per_block;
