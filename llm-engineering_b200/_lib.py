@@ -124,7 +124,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _i32, _f32, _p, _i64, _i64, _p, _sz, _i32, _p, _p],
     ),
     "b2p_paged_prefill_fp8_scratch_size": (
-        _sz, [_i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32],
+        _sz, [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32],
     ),
     "b2p_paged_prefill_fp8": (
         _i32,

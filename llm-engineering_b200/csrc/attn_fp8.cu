@@ -4,10 +4,10 @@
 //
 // Few rows stream the codes (decode_fp8.cu). Many rows are bound by the tensor cores and read
 // every key tile once per 128-row query tile and head pair; there the histories are widened once
-// per call into a 16-bit scratch pool and the 16-bit tile kernel (prefill_tc.cu) runs on that.
-// Widening inside the tile kernel instead, by two more warps that fill its shared-memory tiles
-// from the codes, repeats the conversion for every query tile and head pair: 2351 us against
-// 745 on 32 prompts of 64 to 8192 tokens.
+// per call into a 16-bit scratch pool (22 us of the 750 below) and the 16-bit tile kernel
+// (prefill_tc.cu) runs on that. Widening inside the tile kernel instead, by two more warps that
+// fill its shared-memory tiles from the codes, repeats the conversion for every query tile and
+// head pair: 2351 us against 750 on 32 prompts of 64 to 8192 tokens.
 #include <type_traits>
 
 #include "fp8.cuh"
@@ -40,6 +40,16 @@ int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                    int num_kv_heads, int head_dim, int block_size, float scale, void* out,
                    int64_t out_tok_stride, int64_t out_head_stride, int dtype, int32_t* err_flag,
                    void* stream);
+
+float b2p_prefill_no_weight();
+int b2p_prefill_tc_split(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                         const void* key_cache, const void* value_cache, int64_t num_slots,
+                         const int32_t* block_tables, int64_t block_table_stride,
+                         const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
+                         int64_t total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                         int block_size, float scale, void* out, int64_t out_tok_stride,
+                         int64_t out_head_stride, int dtype, int32_t* err_flag, void* stream,
+                         int splits, float* part, float* lse);
 
 namespace {
 
@@ -75,6 +85,9 @@ struct WidenParams {
   int64_t o_tok, o_head, num_rows;
   int num_seqs, hq, hkv, d, block_size;
   int64_t num_blocks;
+  float* lse;  // split calls: weights to clear, num_lse of them (null: none)
+  int64_t num_lse;
+  float no_weight;
   int32_t* err;
 };
 
@@ -92,6 +105,9 @@ template <typename T>
 __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenParams p) {
   __shared__ int found[2];  // sequence (-1: no block left) and block number
   const int lane = threadIdx.x & 31;
+  for (int64_t i = blockIdx.x * (int64_t)kWidenThreads + threadIdx.x; i < p.num_lse;
+       i += (int64_t)gridDim.x * kWidenThreads)
+    p.lse[i] = p.no_weight;
   // rows before a sequence's first position see nothing: zeros (the tile kernel may skip them)
   for (int seq = blockIdx.x; seq < p.num_seqs; seq += gridDim.x) {
     const int q0 = __ldg(p.cu + seq), rows = __ldg(p.cu + seq + 1) - q0, ctx = __ldg(p.ctx + seq);
@@ -175,11 +191,33 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
   }
 }
 
-// Scratch of the widened form: the block tables, then K, then V.
+constexpr int kMostSplits = 8;
+constexpr int kRunTiles = 8;
+
+// Scratch of the widened form: the block tables, then K, then V, then (split calls) the runs'
+// results and weights.
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
 size_t wide_bytes(int num_seqs, int64_t width, int num_kv_heads, int head_dim, int block_size) {
   return align256((size_t)num_seqs * width * block_size * num_kv_heads * head_dim * 2);
+}
+
+// Runs that every (query tile, pair of heads) item's keys are cut into, where a call has too few
+// items for the SMs: one wave of them where they are fewer than half the SMs, else about three
+// per SM, so that a long history next to short ones does not set the time. A run is at least
+// kRunTiles KV tiles of the longest history that the block tables can hold. Four 512-token
+// slices over 100 to 7777 tokens (14/2 heads): 103 us whole, 88 in two runs, 78 in three, 89 in
+// six; one such slice over 8000 tokens (12/2 heads): 63 in five runs, 83 in eight (a second
+// wave); four whole 512-token prompts: 47 whole, 60 in four runs.
+int key_splits(int num_seqs, int64_t total_q, int64_t table_width, int num_q_heads, int num_kv_heads, int block_size) {
+  const int pairs = (num_q_heads / num_kv_heads + 1) / 2;
+  const int64_t items = ((total_q + 127) / 128 + num_seqs - 1) * num_kv_heads * pairs;
+  const int64_t sms = b2p_host::sm_count();
+  const int64_t most = table_width * block_size / 128 / kRunTiles;
+  int64_t n = items >= 3 * sms ? 1 : items <= sms / 2 ? sms / items : (3 * sms + items - 1) / items;
+  n = n < most ? n : most;
+  n = n < kMostSplits ? n : kMostSplits;
+  return (int)(n > 1 ? n : 1);
 }
 
 bool tile_shape(int head_dim, int block_size, int dtype) {
@@ -247,15 +285,19 @@ extern "C" int b2p_paged_decode_fp8(const void* q, int64_t q_tok_stride, int64_t
                            dtype, err_flag, stream);
 }
 
-extern "C" size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t table_width, int num_q_heads,
+extern "C" size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total_q, int64_t table_width, int num_q_heads,
                                                      int num_kv_heads, int head_dim, int block_size,
                                                      int max_q_len, int dtype) {
-  if (num_seqs <= 0 || table_width <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+  if (num_seqs <= 0 || total_q <= 0 || table_width <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
       block_size <= 0 || max_q_len < 0 || num_q_heads % num_kv_heads != 0 || !tile_shape(head_dim, block_size, dtype))
     return 0;
   if (b2p_rows_fp8_takes(num_q_heads / num_kv_heads, head_dim, block_size, dtype, max_q_len)) return 0;
+  const int splits = key_splits(num_seqs, total_q, table_width, num_q_heads, num_kv_heads, block_size);
+  const size_t parts = splits > 1 ? align256((size_t)splits * total_q * num_q_heads * head_dim * 4) +
+                                        align256((size_t)splits * total_q * num_q_heads * 4)
+                                  : 0;
   return align256((size_t)num_seqs * table_width * 4) +
-         2 * wide_bytes(num_seqs, table_width, num_kv_heads, head_dim, block_size);
+         2 * wide_bytes(num_seqs, table_width, num_kv_heads, head_dim, block_size) + parts;
 }
 
 extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -289,7 +331,7 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
   if (tile_shape(head_dim, block_size, dtype) && aligned(key_cache, 16) && aligned(value_cache, 16) &&
       (int64_t)num_seqs * width * block_size <= 0x7fffffffLL && width > 0 &&
       tile_rows_fit(q, q_tok_stride, q_head_stride, out, out_tok_stride, out_head_stride)) {
-    if (!scratch || scratch_size < b2p_paged_prefill_fp8_scratch_size(num_seqs, width, num_q_heads, num_kv_heads,
+    if (!scratch || scratch_size < b2p_paged_prefill_fp8_scratch_size(num_seqs, total_q, width, num_q_heads, num_kv_heads,
                                                                       head_dim, block_size, max_q_len, dtype) ||
         !aligned(scratch, 16))
       return B2P_EWORKSPACE;
@@ -322,6 +364,12 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     w.block_size = block_size;
     w.num_blocks = num_slots / block_size;
     w.err = err_flag;
+    const int splits = key_splits(num_seqs, total_q, width, num_q_heads, num_kv_heads, block_size);
+    float* part = reinterpret_cast<float*>(base + tables + 2 * pool);
+    w.lse = reinterpret_cast<float*>(base + tables + 2 * pool +
+                                     align256((size_t)splits * total_q * num_q_heads * head_dim * 4));
+    w.num_lse = splits > 1 ? (int64_t)splits * total_q * num_q_heads : 0;
+    w.no_weight = b2p_prefill_no_weight();
     const int64_t most = (int64_t)b2p_host::sm_count() * 8;
     const int64_t blocks = (int64_t)num_seqs * width;
     const unsigned grid = (unsigned)(blocks < most ? blocks : most);
@@ -332,6 +380,12 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
       widen_histories<__half><<<grid, kWidenThreads, 0, s>>>(w);
     const int wrc = b2p_host::check_launch();
     if (wrc != B2P_OK) return wrc;
+    if (splits > 1)
+      return b2p_prefill_tc_split(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1],
+                                  blocks * block_size, w.tables, width, cu_seqlens_q, context_lens,
+                                  num_seqs, total_q, num_q_heads, num_kv_heads, head_dim, block_size,
+                                  scale, out, out_tok_stride, out_head_stride, dtype, err_flag,
+                                  stream, splits, part, w.lse);
     return b2p_prefill_tc(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1], 0, 1,
                           blocks * block_size, w.tables, width, cu_seqlens_q, context_lens,
                           num_seqs, total_q, num_q_heads, num_kv_heads, head_dim, block_size,

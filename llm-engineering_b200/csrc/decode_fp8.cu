@@ -1,5 +1,5 @@
 // Attention of a few query rows per sequence over the 8-bit paged cache (bf16 / f16 queries):
-// the decode step (one row) and the rows of drafted tokens.
+// the decode step (one row), the rows of drafted tokens, short prompt slices.
 //
 //   out[r, h, :] = softmax_t(q[r, h, :] . kc[t] * ks[blk t] * scale, t <= pos(r)) @ (vc[t] * vs[blk t])
 // with e4m3 codes kc, vc and one scale per (block of tokens, KV head). HBM-bound: 2 * head_dim
@@ -1076,7 +1076,11 @@ int64_t fp8_ctas(int num_kv_heads) {
 // that followed the call's own records, one buffer used for calls of one and of five rows in
 // turn would find records where it looks for zeroed counters.)
 constexpr int kMostColumns = 16;   // per virtual sequence
-constexpr int kRowColumns = 64;    // columns per sequence that calls here have at most
+// Columns per sequence that calls here have at most; more belong to the tile kernel, which pays
+// for 128 rows per query tile. 12/2 heads, histories of 512 to 4090 tokens, here against there:
+// 128 sequences of 16 rows (96 columns) 179 us against 378, of 26 rows (156) 281 against 379; four
+// sequences of 26 rows 28 against 47; short histories (20 to 300) of 26 rows 43 against 37.
+constexpr int kRowColumns = 160;
 
 size_t records_bytes(int num_kv_heads) {
   const int64_t ctas = num_kv_heads > b2p_host::sm_count() ? num_kv_heads : b2p_host::sm_count();

@@ -63,6 +63,7 @@ constexpr int kSub = 16;
 constexpr int kSubPerTile = kN / kSub;
 constexpr int kConsumerWarps = 17;  // the MMA issuer and sixteen softmax warps
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr float kNoWeight = -1e30f;        // weight of a run whose keys a row does not see
 
 struct PrefillParams {
   int hq;                  // query heads
@@ -80,6 +81,12 @@ struct PrefillParams {
   uint8_t* out;
   int64_t o_tok, o_head;
   int32_t* err;
+  // split items only: every item's KV tiles in `splits` runs, each with its own fp32 result
+  // O / l in part [splits][rows][hq][D] and weight m + log2(l) in lse [splits][rows][hq]
+  int splits;
+  int64_t num_rows;
+  float* part;
+  float* lse;
 };
 
 // Shared-memory plan (bytes from the 1024-aligned base) for head_dim D (64 or 128): Q, K
@@ -222,7 +229,7 @@ __device__ __forceinline__ float row_exp32(const uint32_t (&r)[32], int base, in
 struct ItemInfo {
   int seq;  // -1: no more work for this CTA
   int qt, kvh, qh_a, qh_b;  // qh_b = -1: head A only
-  int q0, qlen, ctx, rows_valid, pos0, n_kv, pad;
+  int q0, qlen, ctx, rows_valid, pos0, n_kv, run;
 };
 
 __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
@@ -386,7 +393,11 @@ __device__ __forceinline__ bool decode_tile_item(const PrefillParams& p, const S
 // (dynamic, so faster SMs take more items and the short items come last). Tensor memory,
 // barriers and descriptors are set up once; the stage and per-head counters run on across
 // items, so the next item's Q and first K/V tiles load while the current item finishes.
-template <typename T, int D>
+//
+// kSplit: each item is cut into p.splits runs of KV tiles, worked as items of their own (a launch
+// of few query tiles over long histories has too few items for the SMs, and its longest one
+// sets the time); their partial results are merged by the caller.
+template <typename T, int D, bool kSplit>
 __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_constant__ CUtensorMap qmap,
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap,
@@ -475,7 +486,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
     const int64_t total = build_sched_tables(p, st, lane, maxv);
     const int pairs = (p.group + 1) >> 1;
     const int64_t per_tile = (int64_t)(p.hq / p.group) * pairs;
-    const int64_t n_items = total * per_tile;
+    const int64_t n_items = total * per_tile * (kSplit ? p.splits : 1);
     const int spb = p.block_size / kSub;
     const int64_t num_slots = p.num_blocks * p.block_size;
     if (lane == 0) {
@@ -511,10 +522,12 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
       const int64_t k = __shfl_sync(0xffffffffu, claim, 0);
       ItemInfo it;
       it.seq = -1;
+      int kt0 = 0;  // first KV tile of the run
       if (k < n_items && !aborted) {
         int seq = 0, tile = 0;
-        if (decode_tile_item(p, st, k / per_tile, maxv, lane, seq, tile)) {
-          const int r = (int)(k % per_tile);
+        const int64_t item = kSplit ? k / p.splits : k;
+        if (decode_tile_item(p, st, item / per_tile, maxv, lane, seq, tile)) {
+          const int r = (int)(item % per_tile);
           const int pr = r % pairs;
           it.seq = seq;
           it.qt = tile;
@@ -529,6 +542,14 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
           const int last_pos = it.pos0 + it.rows_valid - 1;
           it.n_kv = last_pos >= 0 ? ceil_div(last_pos + 1, kN) : 0;
           if (lane == 0 && (it.ctx < it.qlen || it.n_kv == 0)) set_device_error(p.err, B2P_DEV_LENGTH);
+          if constexpr (kSplit) {  // the run's tiles, positions and keys count from its first tile
+            const int run = (int)(k - item * p.splits);
+            kt0 = (int)((int64_t)it.n_kv * run / p.splits);
+            it.n_kv = (int)((int64_t)it.n_kv * (run + 1) / p.splits) - kt0;
+            it.pos0 -= kt0 * kN;
+            it.ctx = min(it.ctx - kt0 * kN, it.n_kv * kN);
+            it.run = run;
+          }
         }
       }
       const int b = i & 1;
@@ -575,15 +596,16 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
         const int s = (int)(g & 1);
         if (j * kSubPerTile >= win + 32) {
           win = j * kSubPerTile;
-          const int sb = win + lane;  // sub-block index within the sequence
-          const int64_t col = sb / spb;
+          const int sb = win + lane;  // sub-block index within the sequence (or the run)
+          const int at = kSplit ? sb + kt0 * kSubPerTile : sb;
+          const int64_t col = at / spb;
           int32_t blk = -1;
           if ((int64_t)sb * kSub < it.ctx && col < p.bt_stride) blk = __ldg(bt + col);
           if ((int64_t)sb * kSub < it.ctx && (blk < 0 || (int64_t)blk >= p.num_blocks)) {
             set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
             blk = -1;
           }
-          my_slot = (int32_t)(blk < 0 ? num_slots : (int64_t)blk * p.block_size + (int64_t)(sb % spb) * kSub);
+          my_slot = (int32_t)(blk < 0 ? num_slots : (int64_t)blk * p.block_size + (int64_t)(at % spb) * kSub);
         }
         int32_t slots[kSubPerTile];
 #pragma unroll
@@ -971,6 +993,24 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
       uint8_t* stage = smem + L::kOffStage + local * (32 * 32);
       const int64_t row0 = (int64_t)it.q0 + it.qt * kM + quarter * 32;  // this warp's rows
       const int nrows = min(32, it.rows_valid - quarter * 32);
+      if constexpr (kSplit) {  // fp32, each thread its own row's columns
+        const bool mine = lane < nrows;
+        const int64_t at = ((int64_t)it.run * p.num_rows + row0 + lane) * p.hq + qh;
+        if (mine && half == 0) p.lse[at] = lt == 0.f ? kNoWeight : m + __log2f(lt);
+        for (int c0 = 0; c0 < D / 2; c0 += 16) {
+          uint32_t o[16];
+          tmem_ld16(o_col + c0, o);
+          tmem_wait_ld();
+          float4* to = reinterpret_cast<float4*>(p.part + at * D + (D / 2) * half + c0);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (mine)
+              to[c] = make_float4(__uint_as_float(o[4 * c]) * inv, __uint_as_float(o[4 * c + 1]) * inv,
+                                  __uint_as_float(o[4 * c + 2]) * inv, __uint_as_float(o[4 * c + 3]) * inv);
+        }
+        tc_fence_before();
+        continue;
+      }
       T* obase = reinterpret_cast<T*>(p.out) + (int64_t)qh * p.o_head + (D / 2) * half;
       const int sw = (lane >> 2) & 1;
       for (int c0 = 0; c0 < D / 2; c0 += 16) {
@@ -1029,6 +1069,43 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
   }
 }
 
+// Rows of split items: out = sum_s w_s O_s / sum_s w_s, w_s = 2^(lse_s - max). A row that no run
+// wrote (it belongs to no sequence, or sees nothing) is left alone. One thread per 4 head dims.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) merge_splits(const PrefillParams p) {
+  constexpr int kPer = D / 4;
+  const int64_t total = p.num_rows * p.hq * kPer;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t at = i / kPer;  // (row, head)
+    const int c = (int)(i - at * kPer);
+    const int64_t step = p.num_rows * p.hq;
+    float top = kNoWeight;
+    bool any = false;
+    for (int s = 0; s < p.splits; ++s) {
+      const float w = p.lse[s * step + at];
+      any |= w != kNoWeight;
+      top = fmaxf(top, w);
+    }
+    if (!any) continue;
+    float sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+      const float x = p.lse[s * step + at];
+      if (x == kNoWeight) continue;  // not written
+      const float w = fast_exp2(x - top);
+      const float4 v = reinterpret_cast<const float4*>(p.part + (s * step + at) * D)[c];
+      sum += w;
+      o.x = fmaf(w, v.x, o.x);
+      o.y = fmaf(w, v.y, o.y);
+      o.z = fmaf(w, v.z, o.z);
+      o.w = fmaf(w, v.w, o.w);
+    }
+    const float f = 1.f / sum;
+    T* out = reinterpret_cast<T*>(p.out) + (at / p.hq) * p.o_tok + (at % p.hq) * p.o_head + c * 4;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o.x * f, o.y * f), pack2<T>(o.z * f, o.w * f));
+  }
+}
+
 // Claim counters of prefill launches. A launch takes the next of these slots (round robin)
 // and leaves it zeroed, so up to 64 launches can be in flight on a device at once.
 constexpr int kCounterSlots = 64;
@@ -1071,16 +1148,16 @@ int tensor_map_4d_rows(CUtensorMap* out, const void* base, int64_t rows, int hea
                        int box_rows);
 }  // namespace b2p_host
 
-// Launches the tcgen05 prefill when the shape allows it; returns B2P_EUNSUPPORTED otherwise
-// (the caller then runs the CUDA-core kernel).
-int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+namespace {
+
+int launch_prefill(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                    const void* key_cache, const void* value_cache, int64_t layer_index,
                    int64_t num_layers, int64_t num_slots, const int32_t* block_tables,
                    int64_t block_table_stride, const int32_t* cu_seqlens_q,
                    const int32_t* context_lens, int num_seqs, int64_t total_q, int num_q_heads,
                    int num_kv_heads, int head_dim, int block_size, float scale, void* out,
                    int64_t out_tok_stride, int64_t out_head_stride, int dtype, int32_t* err_flag,
-                   void* stream) {
+                   void* stream, int splits, float* part, float* lse) {
   if ((head_dim != 64 && head_dim != 128) || (dtype != B2P_BF16 && dtype != B2P_F16) ||
       block_size % kSub != 0)
     return B2P_EUNSUPPORTED;
@@ -1115,6 +1192,10 @@ int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
   p.o_head = out_head_stride;
   p.err = err_flag;
   p.hq = num_q_heads;
+  p.splits = splits;
+  p.num_rows = total_q;
+  p.part = part;
+  p.lse = lse;
   {
     static std::atomic<uint32_t> next_slot{0};
     int32_t* addr = nullptr;
@@ -1124,18 +1205,22 @@ int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
     p.ctr = addr + 2 * slot;
   }
   const bool bf16 = dtype == B2P_BF16;
-  const int variant = (bf16 ? 0 : 1) + (head_dim == 64 ? 2 : 0);
-  const void* fn =
-      head_dim == 64
-          ? (bf16 ? reinterpret_cast<const void*>(&paged_prefill_tc<__nv_bfloat16, 64>)
-                  : reinterpret_cast<const void*>(&paged_prefill_tc<__half, 64>))
-          : (bf16 ? reinterpret_cast<const void*>(&paged_prefill_tc<__nv_bfloat16, 128>)
-                  : reinterpret_cast<const void*>(&paged_prefill_tc<__half, 128>));
+  const int variant = (bf16 ? 0 : 1) + (head_dim == 64 ? 2 : 0) + (splits > 1 ? 4 : 0);
+  const void* const fns[8] = {
+      reinterpret_cast<const void*>(&paged_prefill_tc<__nv_bfloat16, 128, false>),
+      reinterpret_cast<const void*>(&paged_prefill_tc<__half, 128, false>),
+      reinterpret_cast<const void*>(&paged_prefill_tc<__nv_bfloat16, 64, false>),
+      reinterpret_cast<const void*>(&paged_prefill_tc<__half, 64, false>),
+      reinterpret_cast<const void*>(&paged_prefill_tc<__nv_bfloat16, 128, true>),
+      reinterpret_cast<const void*>(&paged_prefill_tc<__half, 128, true>),
+      reinterpret_cast<const void*>(&paged_prefill_tc<__nv_bfloat16, 64, true>),
+      reinterpret_cast<const void*>(&paged_prefill_tc<__half, 64, true>)};
+  const void* fn = fns[variant];
   const int smem = (head_dim == 64 ? Plan<64>::kSmemBytes : Plan<128>::kSmemBytes) + 1024;
   // Persistent: one CTA per SM walks the work items (its 512 TMEM columns and, for head_dim
   // 128, ~222 KB of shared memory fill the SM). Once per device and kernel variant: the
   // kernel's shared-memory attributes, and whether one CTA fits the SM's limits.
-  static int resident[64][4] = {};
+  static int resident[64][8] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return b2p_host::record_error(e);
@@ -1168,5 +1253,56 @@ int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
   e = cudaLaunchKernel(fn, grid, dim3(kThreads), args, (size_t)smem,
                        static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return b2p_host::record_error(e);
+  const int lrc = b2p_host::check_launch();
+  if (lrc != B2P_OK || splits == 1) return lrc;
+  const int64_t want = (total_q * num_q_heads * (head_dim / 4) + 255) / 256;
+  const int64_t most = (int64_t)b2p_host::sm_count() * 8;
+  const unsigned blocks = (unsigned)(want < most ? want : most);
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (head_dim == 64) {
+    if (bf16) merge_splits<__nv_bfloat16, 64><<<blocks, 256, 0, cs>>>(p);
+    else merge_splits<__half, 64><<<blocks, 256, 0, cs>>>(p);
+  } else {
+    if (bf16) merge_splits<__nv_bfloat16, 128><<<blocks, 256, 0, cs>>>(p);
+    else merge_splits<__half, 128><<<blocks, 256, 0, cs>>>(p);
+  }
   return b2p_host::check_launch();
+}
+
+}  // namespace
+
+// Launches the tcgen05 prefill when the shape allows it; returns B2P_EUNSUPPORTED otherwise
+// (the caller then runs the CUDA-core kernel).
+int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                   const void* key_cache, const void* value_cache, int64_t layer_index,
+                   int64_t num_layers, int64_t num_slots, const int32_t* block_tables,
+                   int64_t block_table_stride, const int32_t* cu_seqlens_q,
+                   const int32_t* context_lens, int num_seqs, int64_t total_q, int num_q_heads,
+                   int num_kv_heads, int head_dim, int block_size, float scale, void* out,
+                   int64_t out_tok_stride, int64_t out_head_stride, int dtype, int32_t* err_flag,
+                   void* stream) {
+  return launch_prefill(q, q_tok_stride, q_head_stride, key_cache, value_cache, layer_index,
+                        num_layers, num_slots, block_tables, block_table_stride, cu_seqlens_q,
+                        context_lens, num_seqs, total_q, num_q_heads, num_kv_heads, head_dim,
+                        block_size, scale, out, out_tok_stride, out_head_stride, dtype, err_flag,
+                        stream, 1, nullptr, nullptr);
+}
+
+// The same with every item's keys in `splits` (> 1) runs: part holds splits * total_q *
+// num_q_heads * head_dim floats, lse splits * total_q * num_q_heads, filled with
+// b2p_prefill_no_weight() by the caller (earlier on the stream).
+float b2p_prefill_no_weight() { return kNoWeight; }
+
+int b2p_prefill_tc_split(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                         const void* key_cache, const void* value_cache, int64_t num_slots,
+                         const int32_t* block_tables, int64_t block_table_stride,
+                         const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
+                         int64_t total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                         int block_size, float scale, void* out, int64_t out_tok_stride,
+                         int64_t out_head_stride, int dtype, int32_t* err_flag, void* stream,
+                         int splits, float* part, float* lse) {
+  return launch_prefill(q, q_tok_stride, q_head_stride, key_cache, value_cache, 0, 1, num_slots,
+                        block_tables, block_table_stride, cu_seqlens_q, context_lens, num_seqs,
+                        total_q, num_q_heads, num_kv_heads, head_dim, block_size, scale, out,
+                        out_tok_stride, out_head_stride, dtype, err_flag, stream, splits, part, lse);
 }

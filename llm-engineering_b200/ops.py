@@ -638,7 +638,8 @@ def paged_prefill_fp8(
     row j of it sits at position ``context_lens[i] - q_len + j``. ``max_q_len`` bounds the q_len
     (rows of a longer sequence are flagged, or computed all the same). Rows of q that no sequence
     owns are left alone in out. Calls of many rows widen the histories into a 16-bit copy of
-    ``num_seqs * block_tables.shape[1]`` blocks of one layer, allocated for the call.
+    ``num_seqs * block_tables.shape[1]`` blocks of one layer, allocated for the call (with fp32
+    partial results where few query tiles are spread over the SMs by their keys).
     """
     index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
                                                      value_scales, block_size)
@@ -648,8 +649,8 @@ def paged_prefill_fp8(
     _vector(index, "cu_seqlens_q", cu_seqlens_q, torch.int32)
     width = _check_tables(index, n, block_tables, context_lens)
     workspace = _fp8_workspace(index, workspace, n, hq, hkv, d, max_q_len)
-    size = _lib.load().b2p_paged_prefill_fp8_scratch_size(n, width, hq, hkv, d, block_size,
-                                                          max_q_len, code)
+    size = _lib.load().b2p_paged_prefill_fp8_scratch_size(n, total_q, width, hq, hkv, d,
+                                                          block_size, max_q_len, code)
     scratch = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     _call("b2p_paged_prefill_fp8", index, q.data_ptr(), qt, qh, key_cache.data_ptr(),
           value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,

@@ -96,8 +96,9 @@ SHAPES = [
     (32, 2, 128, 16),   # group of 16
     (4, 4, 64, 16),     # no GQA
     (6, 2, 128, 48),    # a block size that is not a power of two
+    (20, 1, 64, 16),    # a group of 20: two column passes
     (6, 2, 128, 8),     # CUDA-core kernel: block size below 16
-    (20, 1, 64, 16),    # ... group above 16
+    (200, 1, 64, 16),   # ... group above 160
     (4, 2, 40, 16),     # ... head_dim
     (4, 2, 256, 16),
 ]
@@ -231,6 +232,11 @@ PREFILL = [
     (14, 2, 64, 16, [(0, 129), (300, 70), (0, 5)]),
     (6, 2, 128, 48, [(10, 140), (200, 33)]),
     (5, 5, 64, 64, [(0, 260), (64, 64)]),
+    (12, 2, 128, 16, [(90, 26), (0, 20), (500, 17)]),   # ten passes of 16 columns
+    (2, 2, 64, 32, [(0, 150), (33, 160), (10, 1)]),     # no GQA: 160 rows in as many columns
+    (40, 2, 64, 16, [(70, 3), (0, 4)]),                 # a group of 20
+    (12, 2, 128, 16, [(2300, 130), (5, 200)]),          # the tile kernel with split keys
+    (14, 2, 64, 32, [(4200, 180), (0, 3), (129, 128)]),
     (6, 2, 128, 8, [(10, 40), (0, 3)]),
     (4, 2, 40, 16, [(10, 20), (0, 3)]),
     (4, 2, 256, 16, [(10, 20)]),

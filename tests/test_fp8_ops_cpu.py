@@ -58,9 +58,9 @@ def test_attention_refusals():
     assert decode(d=60) == decode(d=512) == prefill(d=264) == L.B2P_EUNSUPPORTED
     # rows that fit no pass of the few-row kernel need the scratch, few rows the workspace
     assert prefill(rows=200, max_q=200) == decode() == L.B2P_EWORKSPACE
-    assert c.b2p_paged_prefill_fp8_scratch_size(2, 10, 4, 2, 64, 16, 200, 0) >= 2 * 10 * 16 * 2 * 64 * 4
-    assert c.b2p_paged_prefill_fp8_scratch_size(2, 10, 4, 2, 64, 16, 5, 0) == 0
-    assert c.b2p_paged_prefill_fp8_scratch_size(2, 10, 4, 2, 64, 16, 200, 2) == 0
+    assert c.b2p_paged_prefill_fp8_scratch_size(2, 300, 10, 4, 2, 64, 16, 200, 0) >= 2 * 10 * 16 * 2 * 64 * 4
+    assert c.b2p_paged_prefill_fp8_scratch_size(2, 300, 10, 4, 2, 64, 16, 5, 0) == 0
+    assert c.b2p_paged_prefill_fp8_scratch_size(2, 300, 10, 4, 2, 64, 16, 200, 2) == 0
     assert c.b2p_paged_fp8_workspace_size(0, 4, 2, 64, 1) == 0
     assert c.b2p_paged_fp8_workspace_size(4, 12, 2, 128, 1) > 0
 
