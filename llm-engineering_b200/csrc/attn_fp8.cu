@@ -81,6 +81,8 @@ struct WidenParams {
   int width;
   const int32_t* cu;
   const int32_t* ctx;
+  int32_t* safe_cu;   // [num_seqs + 1] and [num_seqs]: the same within q's rows and the tables'
+  int32_t* safe_ctx;  // reach, for the tile kernel, which trusts them
   uint8_t* out;
   int64_t o_tok, o_head, num_rows;
   int num_seqs, hq, hkv, d, block_size;
@@ -97,6 +99,10 @@ __device__ __forceinline__ float bounded(float x) {
   return std::is_same<T, __half>::value ? (x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x) : x;
 }
 
+__device__ __forceinline__ int row_within(const WidenParams& p, int row) {
+  return (int)min(max((int64_t)row, (int64_t)0), p.num_rows);
+}
+
 // A CTA takes the used blocks of all histories in turn (found by a scan of the lengths, 32
 // sequences at a time: with one CTA per table entry, most of a ragged batch's are empty, 35 us
 // against 17 on 32 prompts) and writes their codes as 16-bit rows into the scratch block that the
@@ -110,17 +116,20 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
     p.lse[i] = p.no_weight;
   // rows before a sequence's first position see nothing: zeros (the tile kernel may skip them)
   for (int seq = blockIdx.x; seq < p.num_seqs; seq += gridDim.x) {
-    const int q0 = __ldg(p.cu + seq), rows = __ldg(p.cu + seq + 1) - q0, ctx = __ldg(p.ctx + seq);
+    const int first = __ldg(p.cu + seq), last = __ldg(p.cu + seq + 1), ctx = __ldg(p.ctx + seq);
+    const int q0 = row_within(p, first), rows = row_within(p, last) - q0;
     const int blind = min(rows, rows - max(ctx, 0));
-    if (threadIdx.x == 0 && rows > 0) {
-      if (blind > 0) set_device_error(p.err, B2P_DEV_LENGTH);
-      if (ctx > (int64_t)p.width * p.block_size) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
+    if (threadIdx.x == 0) {
+      if (q0 != first || q0 + rows != last || (rows > 0 && blind > 0)) set_device_error(p.err, B2P_DEV_LENGTH);
+      if (rows > 0 && ctx > (int64_t)p.width * p.block_size) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
+      p.safe_cu[seq] = q0;
+      if (seq == p.num_seqs - 1) p.safe_cu[seq + 1] = q0 + rows;
+      p.safe_ctx[seq] = (int)min((int64_t)ctx, (int64_t)p.width * p.block_size);
     }
     for (int64_t e = threadIdx.x; e < (int64_t)max(blind, 0) * p.hq * p.d; e += kWidenThreads) {
       const int64_t row = q0 + e / (p.hq * p.d);
       const int r = (int)(e % (p.hq * p.d));
-      if (row >= 0 && row < p.num_rows)
-        reinterpret_cast<T*>(p.out)[row * p.o_tok + (int64_t)(r / p.d) * p.o_head + r % p.d] = from_f32<T>(0.f);
+      reinterpret_cast<T*>(p.out)[row * p.o_tok + (int64_t)(r / p.d) * p.o_head + r % p.d] = from_f32<T>(0.f);
     }
   }
   for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
@@ -132,7 +141,8 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
         const int s = base + lane;
         int n = 0;
         if (s < p.num_seqs && __ldg(p.cu + s + 1) > __ldg(p.cu + s))
-          n = min(p.width, (max(__ldg(p.ctx + s), 0) + p.block_size - 1) / p.block_size);
+          n = (int)min((int64_t)p.width,
+                       ((int64_t)max(__ldg(p.ctx + s), 0) + p.block_size - 1) / p.block_size);
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -194,8 +204,8 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
 constexpr int kMostSplits = 8;
 constexpr int kRunTiles = 8;
 
-// Scratch of the widened form: the block tables, then K, then V, then (split calls) the runs'
-// results and weights.
+// Scratch of the widened form: the block tables with the checked offsets and lengths, then K, then
+// V, then (split calls) the runs' results and weights.
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
 size_t wide_bytes(int num_seqs, int64_t width, int num_kv_heads, int head_dim, int block_size) {
@@ -225,7 +235,8 @@ bool tile_shape(int head_dim, int block_size, int dtype) {
          (dtype == B2P_BF16 || dtype == B2P_F16);
 }
 
-int check_args(const void* key_cache, const void* value_cache, int64_t layer_index, int64_t num_layers, int64_t num_slots, int num_seqs,
+int check_args(const void* key_cache, const void* value_cache, const void* workspace, float scale,
+               int64_t layer_index, int64_t num_layers, int64_t num_slots, int num_seqs,
                int64_t num_rows, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
                int block_size, int64_t block_table_stride, int dtype) {
   if (num_seqs < 0 || num_rows < 0 || max_q_len < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
@@ -235,8 +246,8 @@ int check_args(const void* key_cache, const void* value_cache, int64_t layer_ind
   if (num_q_heads % num_kv_heads != 0 || num_slots % block_size != 0) return B2P_EINVAL;
   if (dtype < B2P_BF16 || dtype > B2P_F32) return B2P_EINVAL;
   if (layer_index < 0 || layer_index >= num_layers) return B2P_ERANGE;
-  if ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 7u)
-    return B2P_EINVAL;
+  if (!aligned(key_cache, 8) || !aligned(value_cache, 8) || !aligned(workspace, 16)) return B2P_EINVAL;
+  if (!(scale >= 0.f)) return B2P_EINVAL;  // the running maxima take a larger product for a larger score
   if (head_dim % 8 != 0 || head_dim > 256 || num_slots > 0x7fffffffLL || num_rows > 0x7fffffffLL)
     return B2P_EUNSUPPORTED;
   return B2P_OK;
@@ -263,7 +274,7 @@ extern "C" int b2p_paged_decode_fp8(const void* q, int64_t q_tok_stride, int64_t
                                     void* out, int64_t out_tok_stride, int64_t out_head_stride,
                                     void* workspace, size_t workspace_size, int dtype,
                                     int32_t* err_flag, void* stream) {
-  const int rc = check_args(key_cache, value_cache, layer_index, num_layers, num_slots, num_seqs, num_seqs, 1, num_q_heads,
+  const int rc = check_args(key_cache, value_cache, workspace, scale, layer_index, num_layers, num_slots, num_seqs, num_seqs, 1, num_q_heads,
                             num_kv_heads, head_dim, block_size, block_table_stride, dtype);
   if (rc != B2P_OK || num_seqs == 0) return rc;
   if (!q || !key_cache || !value_cache || !key_scales || !value_scales || !block_tables ||
@@ -296,7 +307,7 @@ extern "C" size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total
   const size_t parts = splits > 1 ? align256((size_t)splits * total_q * num_q_heads * head_dim * 4) +
                                         align256((size_t)splits * total_q * num_q_heads * 4)
                                   : 0;
-  return align256((size_t)num_seqs * table_width * 4) +
+  return align256(((size_t)num_seqs * table_width + 2 * (size_t)num_seqs + 1) * 4) +
          2 * wide_bytes(num_seqs, table_width, num_kv_heads, head_dim, block_size) + parts;
 }
 
@@ -312,7 +323,7 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
                                      void* workspace, size_t workspace_size, void* scratch,
                                      size_t scratch_size, int dtype,
                                      int32_t* err_flag, void* stream) {
-  const int rc = check_args(key_cache, value_cache, layer_index, num_layers, num_slots, num_seqs, total_q, max_q_len,
+  const int rc = check_args(key_cache, value_cache, workspace, scale, layer_index, num_layers, num_slots, num_seqs, total_q, max_q_len,
                             num_q_heads, num_kv_heads, head_dim, block_size, block_table_stride,
                             dtype);
   if (rc != B2P_OK || num_seqs == 0 || total_q == 0 || max_q_len == 0) return rc;
@@ -343,9 +354,11 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     w.scales[0] = key_scales + layer_index * layer_scales;
     w.scales[1] = value_scales + layer_index * layer_scales;
     uint8_t* base = static_cast<uint8_t*>(scratch);
-    const size_t tables = align256((size_t)num_seqs * width * 4);
+    const size_t tables = align256(((size_t)num_seqs * width + 2 * (size_t)num_seqs + 1) * 4);
     const size_t pool = wide_bytes(num_seqs, width, num_kv_heads, head_dim, block_size);
     w.tables = reinterpret_cast<int32_t*>(base);
+    w.safe_cu = w.tables + num_seqs * width;
+    w.safe_ctx = w.safe_cu + num_seqs + 1;
     w.wide[0] = base + tables;
     w.wide[1] = base + tables + pool;
     w.block_tables = block_tables;
@@ -382,13 +395,13 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     if (wrc != B2P_OK) return wrc;
     if (splits > 1)
       return b2p_prefill_tc_split(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1],
-                                  blocks * block_size, w.tables, width, cu_seqlens_q, context_lens,
-                                  num_seqs, total_q, num_q_heads, num_kv_heads, head_dim, block_size,
+                                  blocks * block_size, w.tables, width, w.safe_cu, w.safe_ctx, num_seqs,
+                                  total_q, num_q_heads, num_kv_heads, head_dim, block_size,
                                   scale, out, out_tok_stride, out_head_stride, dtype, err_flag,
                                   stream, splits, part, w.lse);
     return b2p_prefill_tc(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1], 0, 1,
-                          blocks * block_size, w.tables, width, cu_seqlens_q, context_lens,
-                          num_seqs, total_q, num_q_heads, num_kv_heads, head_dim, block_size,
+                          blocks * block_size, w.tables, width, w.safe_cu, w.safe_ctx, num_seqs,
+                          total_q, num_q_heads, num_kv_heads, head_dim, block_size,
                           scale, out, out_tok_stride, out_head_stride, dtype, err_flag, stream);
   }
   if (dtype != B2P_F32) b2p_host::note_fallback(3);

@@ -73,7 +73,9 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_fp8_simt(const SimtFp8
 #pragma unroll
   for (int k = 0; k < kMaxD / 32; ++k) acc[k] = 0.f;
   const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
-  const int nkeys = pos + 1;
+  const int64_t reach = p.bt_stride * p.block_size;  // what the table's row names
+  const int nkeys = (int)min((int64_t)pos + 1, reach);
+  if (pos >= reach && lane == 0) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
   for (int base = 0; base < nkeys; base += 32) {
     const int t = base + lane;
     float s = -INFINITY, vs = 0.f;

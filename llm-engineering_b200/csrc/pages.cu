@@ -244,6 +244,7 @@ extern "C" int b2p_compact_blocks(void* key_cache, void* value_cache, float* key
   if (!key_cache || !value_cache || !new_ids || !num_live ||
       (num_seqs > 0 && table_width > 0 && (!block_tables || !context_lens)))
     return B2P_EINVAL;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15u) return B2P_EINVAL;
   if (!workspace || workspace_size < b2p_compact_blocks_workspace_size(g.num_blocks))
     return B2P_EWORKSPACE;
   const size_t bits_bytes = align256((size_t)(g.num_blocks + 31) / 32 * 4);

@@ -84,6 +84,8 @@ class PagedKVStorage:
         lists = list(block_table.tables().values())
         if block_table.block_size != self.block_size or block_table.pool.num_blocks != self.num_blocks:
             raise ValueError("block_table must be over this pool's blocks.")
+        if len({b for t in lists for b in t}) != block_table.pool.num_allocated_blocks:
+            raise ValueError("blocks are allocated that no request of block_table holds.")
         width = max([1, *(len(t) for t in lists)])
         host = np.full((len(lists) + 1, width), -1, dtype=np.int32)
         for row, t in zip(host, lists):

@@ -76,6 +76,11 @@ def test_storage_refusals():
     s.copy_blocks([], [])
     with pytest.raises(ValueError, match="this pool"):
         s.compact(table(blocks=10, bs=16))
+    t = table(blocks=4, bs=16)
+    t.allocate_for_request("a", 20)
+    t.pool.allocate(1)  # held by nobody's table: it would be taken for free
+    with pytest.raises(ValueError, match="no request"):
+        s.compact(t)
     f = Fp8PagedKVStorage(2, 4, 16, 1, 8, dev)
     assert f.key_cache.dtype == torch.float8_e4m3fn and f.key_scales.shape == (2, 4, 1)
     with pytest.raises(ValueError, match="append"):

@@ -306,6 +306,48 @@ def test_prefill_flags_what_does_not_fit(ops, long):
     assert (got[:2] == 0).all() and err.item() == 8
 
 
+@pytest.mark.parametrize("shape", [(12, 2, 128, 16), (4, 2, 40, 16)])
+def test_a_context_beyond_its_table_is_cut_and_flagged(ops, shape):
+    """Lengths of 2^31 - 1: what the table names is attended, nothing else is read, no call runs on."""
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(13)
+    tables, bt, blocks = tables_for(rng, [64, 30], bs)
+    pool = Pool(rng, 1, blocks, bs, hkv, d)
+    q = torch.from_numpy(rng.standard_normal((2, hq, d))).to(torch.float16)
+    ctx = torch.tensor([2 ** 31 - 1, 30], dtype=torch.int32, device="cuda")
+    for max_q, cu in ((1, None), (1, [0, 1, 2]), (200, [0, 1, 2])):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        if cu is None:
+            got = ops.paged_decode_fp8(q.cuda(), *pool.device(), 0, bt.cuda(), ctx, bs, d ** -0.5, err_flag=err)
+        else:
+            got = ops.paged_prefill_fp8(q.cuda(), *pool.device(), 0, bt.cuda(),
+                                        torch.tensor(cu, dtype=torch.int32, device="cuda"), ctx, max_q, bs,
+                                        d ** -0.5, err_flag=err)
+        want = ref.attend(q, pool.k[0], pool.ks[0], pool.v[0], pool.vs[0], bs, tables, [1, 1], [64, 30], d ** -0.5)
+        check(got, want, torch.float16, d, 64, p_step(torch.float16, True))
+        assert err.item() == 2
+
+
+@pytest.mark.parametrize("max_q", [4, 300])
+def test_offsets_outside_the_rows_write_nothing_there(ops, max_q):
+    hq, hkv, d, bs = 12, 2, 128, 16
+    rng = np.random.default_rng(14)
+    ctx = [40, 50, 60]
+    tables, bt, blocks = tables_for(rng, ctx, bs)
+    pool = Pool(rng, 1, blocks, bs, hkv, d)
+    q = torch.from_numpy(rng.standard_normal((8, hq, d))).to(torch.bfloat16)
+    out = torch.full((16, hq, d), 5.0, dtype=torch.bfloat16, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.paged_prefill_fp8(q.cuda()[:8], *pool.device(), 0, bt.cuda(),
+                          torch.tensor([0, 3, 6, 10], dtype=torch.int32, device="cuda"),
+                          torch.tensor(ctx, dtype=torch.int32, device="cuda"), max_q, bs, d ** -0.5,
+                          out=out[4:12], err_flag=err)
+    assert err.item() == 8 and (out[:4] == 5).all() and (out[12:] == 5).all()
+    want = ref.attend(q[:6], pool.k[0], pool.ks[0], pool.v[0], pool.vs[0], bs, tables[:2], [3, 3], ctx[:2],
+                      d ** -0.5)
+    check(out[4:10], want, torch.bfloat16, d, 50, p_step(torch.bfloat16, True))
+
+
 # ------------------------------------------------------------------ rows in and out
 WRITES = [
     # (hkv, d, bs, [(past, q_len)])

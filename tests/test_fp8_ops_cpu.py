@@ -43,9 +43,9 @@ def test_write_and_read_refusals():
 def test_attention_refusals():
     L, c = lib()
 
-    def decode(n=1, hq=4, hkv=2, d=64, bs=16, layer=0, q=FAKE, dtype=0, slots=64, cache=FAKE):
+    def decode(n=1, hq=4, hkv=2, d=64, bs=16, layer=0, q=FAKE, dtype=0, slots=64, cache=FAKE, scale=0.1, ws=None):
         return c.b2p_paged_decode_fp8(q, 256, 64, cache, FAKE, FAKE, FAKE, layer, 1, slots, FAKE, 4, FAKE, n, hq,
-                                      hkv, d, bs, 0.1, FAKE, 256, 64, None, 0, dtype, None, None)
+                                      hkv, d, bs, scale, FAKE, 256, 64, ws, 0, dtype, None, None)
 
     def prefill(n=1, rows=2, max_q=2, hq=4, hkv=2, d=64, q=FAKE):
         return c.b2p_paged_prefill_fp8(q, 256, 64, FAKE, FAKE, FAKE, FAKE, 0, 1, 64, FAKE, 4, FAKE, FAKE, n, rows,
@@ -54,6 +54,7 @@ def test_attention_refusals():
     assert decode(n=0) == prefill(n=0) == prefill(rows=0) == prefill(max_q=0) == L.B2P_OK
     assert decode(layer=3) == L.B2P_ERANGE
     assert decode(hq=5) == decode(slots=60) == decode(q=None) == decode(dtype=9) == L.B2P_EINVAL
+    assert decode(scale=-0.1) == decode(scale=float("nan")) == decode(ws=FAKE + 4) == L.B2P_EINVAL
     assert decode(cache=FAKE + 1) == prefill(q=None) == prefill(max_q=-1) == L.B2P_EINVAL
     assert decode(d=60) == decode(d=512) == prefill(d=264) == L.B2P_EUNSUPPORTED
     # rows that fit no pass of the few-row kernel need the scratch, few rows the workspace
@@ -99,6 +100,7 @@ def test_page_refusals():
                                     FAKE, FAKE, ws, size, None, None)
 
     assert compact(stride=3) == compact(tables=None) == compact(n=-1) == L.B2P_EINVAL
+    assert compact(ws=FAKE + 8) == L.B2P_EINVAL
     assert compact(ws=None) == compact(size=16) == L.B2P_EWORKSPACE
     assert c.b2p_compact_blocks_workspace_size(0) == 0
     assert c.b2p_compact_blocks_workspace_size(1 << 20) >= (1 << 17) + (1 << 22)

@@ -131,6 +131,59 @@ def test_speculative_steps_with_forks_and_compaction(ops, dtype):
     assert err.item() == 0
 
 
+def test_offsets_past_32_bits(ops):
+    """A pool of 4.9 GB a tensor whose used blocks lie at its end: every entry point's byte offsets
+    pass 2^32 (the few-row kernel, the tile kernel over the widened copy, rows in and out, copies,
+    and verification rows past 2^31 elements)."""
+    from test_fp8_cache_gpu import check, p_step
+
+    hq, hkv, d, bs, blocks = 28, 4, 128, 16, 600_000
+    rng = np.random.default_rng(1)
+    storage = Fp8PagedKVStorage(1, blocks, bs, hkv, d, DEV)
+    tables = [[blocks - 1 - 3 * i for i in range(12)], [blocks - 2 - 3 * i for i in range(2)]]
+    ctx = [190, 31]
+    bt = i32([tables[0], tables[1] + [-1] * 10])
+    cu = i32([0, 190, 221])
+    k, v = (torch.from_numpy(rng.standard_normal((221, hkv, d))).to(torch.bfloat16) for _ in range(2))
+    storage.append(0, bt, cu, i32(ctx), 190, k.cuda(), v.cuda())
+    ids = sorted(b for t in tables for b in t)
+    small = {b: i for i, b in enumerate(ids)}  # the same blocks in a pool of their own
+    codes, scales = ([np.zeros((len(ids) * bs, hkv, d), np.uint8) for _ in range(2)],
+                     [np.zeros((len(ids), hkv)) for _ in range(2)])
+    own = [[small[b] for b in t] for t in tables]
+    for c, s, x in zip(codes, scales, (k, v)):
+        ref.write(c, s, bs, own, ctx, ctx, x.double().numpy())
+    plain = (torch.from_numpy(codes[0]), torch.from_numpy(scales[0]), torch.from_numpy(codes[1]),
+             torch.from_numpy(scales[1]))
+    slots = [tables[0][p // bs] * bs + p % bs for p in range(190)]
+    got = storage.gather(0, slots)
+    for x, c, s in zip(got, codes, scales):
+        at = np.array([own[0][p // bs] * bs + p % bs for p in range(190)])
+        assert torch.equal(x.double().cpu(), torch.from_numpy(ref.VALUES[c[at]] * s[at // bs][:, :, None]))
+    pool = (storage.key_cache, storage.value_cache, storage.key_scales, storage.value_scales, 0, bt)
+    q = torch.from_numpy(rng.standard_normal((221, hq, d))).to(torch.bfloat16)
+    got = ops.paged_prefill_fp8(q.cuda(), *pool, cu, i32(ctx), 190, bs, d ** -0.5)
+    rows = [0, 17, 100, 189, 190, 220]  # of all rows: enough for the offsets
+    want = ref.attend(q, *plain, bs, own, ctx, ctx, d ** -0.5)
+    check(got[rows], tuple(t[rows] for t in want), torch.bfloat16, d, 190, p_step(torch.bfloat16, True))
+    last = torch.stack([q[189], q[220]])
+    got = ops.paged_decode_fp8(last.cuda(), *pool, i32(ctx), bs, d ** -0.5)
+    check(got, tuple(t[[189, 220]] for t in want), torch.bfloat16, d, 190, p_step(torch.bfloat16, False))
+    storage.copy_blocks([tables[0][0]], [5])
+    assert torch.equal(storage.key_cache[0, 80:96].view(torch.uint8).cpu(), plain[0][own[0][0] * bs:own[0][0] * bs + bs])
+    del storage, got, pool
+    vocab = 151936
+    target = torch.zeros((14200, vocab), dtype=torch.bfloat16, device=DEV)  # 2.16e9 elements
+    target[14199, 77] = 1.0
+    target[:14199, 3] = 1.0
+    n = 14199
+    tokens, accepted = ops.verify_drafts(target, torch.full((1,), 3, dtype=torch.int64, device=DEV),
+                                         i32([0] * n + [1])[:n + 1], torch.zeros(1, device=DEV),
+                                         torch.full((n,), 0.5, device=DEV), 1)
+    assert accepted.tolist() == [0] * (n - 1) + [1]
+    assert tokens[-1].tolist() == [3, 77] and tokens[0].tolist() == [3, -1]
+
+
 def small_model(dtype, seed=0):
     from transformers import Qwen2Config, Qwen2ForCausalLM
 
