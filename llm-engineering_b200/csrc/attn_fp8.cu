@@ -32,24 +32,15 @@ int b2p_rows_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, con
                  void* out, int64_t out_tok_stride, int64_t out_head_stride, void* workspace,
                  size_t workspace_size, int dtype, int32_t* err_flag, void* stream);
 
-int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
-                   const void* key_cache, const void* value_cache, int64_t layer_index,
-                   int64_t num_layers, int64_t num_slots, const int32_t* block_tables,
-                   int64_t block_table_stride, const int32_t* cu_seqlens_q,
-                   const int32_t* context_lens, int num_seqs, int64_t total_q, int num_q_heads,
-                   int num_kv_heads, int head_dim, int block_size, float scale, void* out,
-                   int64_t out_tok_stride, int64_t out_head_stride, int dtype, int32_t* err_flag,
-                   void* stream);
-
 float b2p_prefill_no_weight();
-int b2p_prefill_tc_split(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
-                         const void* key_cache, const void* value_cache, int64_t num_slots,
-                         const int32_t* block_tables, int64_t block_table_stride,
-                         const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
-                         int64_t total_q, int num_q_heads, int num_kv_heads, int head_dim,
-                         int block_size, float scale, void* out, int64_t out_tok_stride,
-                         int64_t out_head_stride, int dtype, int32_t* err_flag, void* stream,
-                         int splits, float* part, float* lse);
+int b2p_prefill_tc_runs(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                        const void* key_cache, const void* value_cache, int64_t num_slots,
+                        const int32_t* block_tables, int64_t block_table_stride,
+                        const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
+                        int64_t total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                        int block_size, float scale, void* out, int64_t out_tok_stride,
+                        int64_t out_head_stride, int dtype, int32_t* err_flag, void* stream,
+                        int32_t* claims, int splits, float* part, float* lse);
 
 namespace {
 
@@ -83,6 +74,7 @@ struct WidenParams {
   const int32_t* ctx;
   int32_t* safe_cu;   // [num_seqs + 1] and [num_seqs]: the same within q's rows and the tables'
   int32_t* safe_ctx;  // reach, for the tile kernel, which trusts them
+  int32_t* claims;    // the tile kernel's two claim counters, to zero
   uint8_t* out;
   int64_t o_tok, o_head, num_rows;
   int num_seqs, hq, hkv, d, block_size;
@@ -105,12 +97,13 @@ __device__ __forceinline__ int row_within(const WidenParams& p, int row) {
 
 // A CTA takes the used blocks of all histories in turn (found by a scan of the lengths, 32
 // sequences at a time: with one CTA per table entry, most of a ragged batch's are empty, 35 us
-// against 17 on 32 prompts) and writes their codes as 16-bit rows into the scratch block that the
+// against 22 on 32 prompts) and writes their codes as 16-bit rows into the scratch block that the
 // scratch table gives them. Memory-bound: 1 byte read and 2 written per element.
 template <typename T>
 __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenParams p) {
   __shared__ int found[2];  // sequence (-1: no block left) and block number
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && threadIdx.x < 2) p.claims[threadIdx.x] = 0;
   for (int64_t i = blockIdx.x * (int64_t)kWidenThreads + threadIdx.x; i < p.num_lse;
        i += (int64_t)gridDim.x * kWidenThreads)
     p.lse[i] = p.no_weight;
@@ -204,9 +197,13 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
 constexpr int kMostSplits = 8;
 constexpr int kRunTiles = 8;
 
-// Scratch of the widened form: the block tables with the checked offsets and lengths, then K, then
-// V, then (split calls) the runs' results and weights.
+// Scratch of the widened form: the block tables with the checked offsets and lengths and the claim
+// counters, then K, then V, then (split calls) the runs' results and weights.
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+size_t table_bytes(int num_seqs, int64_t width) {
+  return align256(((size_t)num_seqs * width + 2 * (size_t)num_seqs + 1 + 2) * 4);
+}
 
 size_t wide_bytes(int num_seqs, int64_t width, int num_kv_heads, int head_dim, int block_size) {
   return align256((size_t)num_seqs * width * block_size * num_kv_heads * head_dim * 2);
@@ -307,7 +304,7 @@ extern "C" size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total
   const size_t parts = splits > 1 ? align256((size_t)splits * total_q * num_q_heads * head_dim * 4) +
                                         align256((size_t)splits * total_q * num_q_heads * 4)
                                   : 0;
-  return align256(((size_t)num_seqs * table_width + 2 * (size_t)num_seqs + 1) * 4) +
+  return table_bytes(num_seqs, table_width) +
          2 * wide_bytes(num_seqs, table_width, num_kv_heads, head_dim, block_size) + parts;
 }
 
@@ -354,11 +351,12 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     w.scales[0] = key_scales + layer_index * layer_scales;
     w.scales[1] = value_scales + layer_index * layer_scales;
     uint8_t* base = static_cast<uint8_t*>(scratch);
-    const size_t tables = align256(((size_t)num_seqs * width + 2 * (size_t)num_seqs + 1) * 4);
+    const size_t tables = table_bytes(num_seqs, width);
     const size_t pool = wide_bytes(num_seqs, width, num_kv_heads, head_dim, block_size);
     w.tables = reinterpret_cast<int32_t*>(base);
     w.safe_cu = w.tables + num_seqs * width;
     w.safe_ctx = w.safe_cu + num_seqs + 1;
+    w.claims = w.safe_ctx + num_seqs;
     w.wide[0] = base + tables;
     w.wide[1] = base + tables + pool;
     w.block_tables = block_tables;
@@ -393,16 +391,11 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
       widen_histories<__half><<<grid, kWidenThreads, 0, s>>>(w);
     const int wrc = b2p_host::check_launch();
     if (wrc != B2P_OK) return wrc;
-    if (splits > 1)
-      return b2p_prefill_tc_split(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1],
-                                  blocks * block_size, w.tables, width, w.safe_cu, w.safe_ctx, num_seqs,
-                                  total_q, num_q_heads, num_kv_heads, head_dim, block_size,
-                                  scale, out, out_tok_stride, out_head_stride, dtype, err_flag,
-                                  stream, splits, part, w.lse);
-    return b2p_prefill_tc(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1], 0, 1,
-                          blocks * block_size, w.tables, width, w.safe_cu, w.safe_ctx, num_seqs,
-                          total_q, num_q_heads, num_kv_heads, head_dim, block_size,
-                          scale, out, out_tok_stride, out_head_stride, dtype, err_flag, stream);
+    return b2p_prefill_tc_runs(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1],
+                               blocks * block_size, w.tables, width, w.safe_cu, w.safe_ctx, num_seqs,
+                               total_q, num_q_heads, num_kv_heads, head_dim, block_size, scale, out,
+                               out_tok_stride, out_head_stride, dtype, err_flag, stream, w.claims,
+                               splits, part, w.lse);
   }
   if (dtype != B2P_F32) b2p_host::note_fallback(3);
   return b2p_attn_fp8_simt(q, q_tok_stride, q_head_stride, key_cache, value_cache, key_scales,

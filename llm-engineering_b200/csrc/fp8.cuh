@@ -17,7 +17,6 @@ namespace b2p {
 // Smallest block exponent. Blocks of smaller values (all-zero ones among them) use it: 448 *
 // 2^-110 is still a normal fp32 number and so are the products with it.
 constexpr int kFp8MinExp = -110;
-constexpr float kFp8Max = 448.f;
 
 // The exponent e of a block's scale 2^e: the smallest e >= kFp8MinExp with amax <= 448 * 2^e.
 // 448 = 1.75 * 2^8, so e is amax's own exponent less 8, plus one where its mantissa is above
@@ -52,10 +51,5 @@ __device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint16_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
 }
-
-// Amax of a row set is tracked on absolute values; a NaN or an infinity in any row makes the
-// block's scale NaN, so that whatever attends the block shows it, as it would over a 16-bit
-// cache. fp8_bad() marks such a value.
-__device__ __forceinline__ bool fp8_bad(float x) { return !(fabsf(x) <= 3.402823466e38f); }
 
 }  // namespace b2p

@@ -1157,7 +1157,7 @@ int launch_prefill(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                    const int32_t* context_lens, int num_seqs, int64_t total_q, int num_q_heads,
                    int num_kv_heads, int head_dim, int block_size, float scale, void* out,
                    int64_t out_tok_stride, int64_t out_head_stride, int dtype, int32_t* err_flag,
-                   void* stream, int splits, float* part, float* lse) {
+                   void* stream, int splits, float* part, float* lse, int32_t* claims) {
   if ((head_dim != 64 && head_dim != 128) || (dtype != B2P_BF16 && dtype != B2P_F16) ||
       block_size % kSub != 0)
     return B2P_EUNSUPPORTED;
@@ -1196,7 +1196,8 @@ int launch_prefill(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
   p.num_rows = total_q;
   p.part = part;
   p.lse = lse;
-  {
+  p.ctr = claims;
+  if (claims == nullptr) {
     static std::atomic<uint32_t> next_slot{0};
     int32_t* addr = nullptr;
     const int crc = prefill_counter_base(&addr);
@@ -1285,24 +1286,27 @@ int b2p_prefill_tc(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                         num_layers, num_slots, block_tables, block_table_stride, cu_seqlens_q,
                         context_lens, num_seqs, total_q, num_q_heads, num_kv_heads, head_dim,
                         block_size, scale, out, out_tok_stride, out_head_stride, dtype, err_flag,
-                        stream, 1, nullptr, nullptr);
+                        stream, 1, nullptr, nullptr, nullptr);
 }
 
-// The same with every item's keys in `splits` (> 1) runs: part holds splits * total_q *
-// num_q_heads * head_dim floats, lse splits * total_q * num_q_heads, filled with
-// b2p_prefill_no_weight() by the caller (earlier on the stream).
+// The same for a caller with scratch of its own. claims: the launch's claim counters, two words
+// that are zero (earlier on the stream): unlike the slots above they are the call's own, so that
+// any number of captured calls may run side by side. splits > 1: every item's keys in that many
+// runs; part holds splits * total_q * num_q_heads * head_dim floats, lse splits * total_q *
+// num_q_heads, filled with b2p_prefill_no_weight() (earlier on the stream).
 float b2p_prefill_no_weight() { return kNoWeight; }
 
-int b2p_prefill_tc_split(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
-                         const void* key_cache, const void* value_cache, int64_t num_slots,
-                         const int32_t* block_tables, int64_t block_table_stride,
-                         const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
-                         int64_t total_q, int num_q_heads, int num_kv_heads, int head_dim,
-                         int block_size, float scale, void* out, int64_t out_tok_stride,
-                         int64_t out_head_stride, int dtype, int32_t* err_flag, void* stream,
-                         int splits, float* part, float* lse) {
+int b2p_prefill_tc_runs(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                        const void* key_cache, const void* value_cache, int64_t num_slots,
+                        const int32_t* block_tables, int64_t block_table_stride,
+                        const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
+                        int64_t total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                        int block_size, float scale, void* out, int64_t out_tok_stride,
+                        int64_t out_head_stride, int dtype, int32_t* err_flag, void* stream,
+                        int32_t* claims, int splits, float* part, float* lse) {
   return launch_prefill(q, q_tok_stride, q_head_stride, key_cache, value_cache, 0, 1, num_slots,
                         block_tables, block_table_stride, cu_seqlens_q, context_lens, num_seqs,
                         total_q, num_q_heads, num_kv_heads, head_dim, block_size, scale, out,
-                        out_tok_stride, out_head_stride, dtype, err_flag, stream, splits, part, lse);
+                        out_tok_stride, out_head_stride, dtype, err_flag, stream, splits, part, lse,
+                        claims);
 }

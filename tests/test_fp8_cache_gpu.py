@@ -520,3 +520,44 @@ def test_a_second_stream_and_a_captured_step(ops):
             want = ref.attend(qh, k8, ks, v8, vs, bs, tables, [1] * 3, ctx, d ** -0.5)
             check(out, want, torch.bfloat16, d, max(ctx), p_step(torch.bfloat16, False))
     torch.cuda.current_stream().wait_stream(side)
+
+
+def test_captured_prompts_replayed_side_by_side(ops):
+    """Two captured calls, 64 calls apart, replayed at once on two streams: nothing that one of them
+    counts in may be the other's."""
+    hq, hkv, d, bs = 12, 2, 128, 16
+    rng = np.random.default_rng(11)
+    q_lens, ctx = [400, 700, 333], [1500, 700, 2000]
+    tables, bt, blocks = tables_for(rng, ctx, bs)
+    pool = Pool(rng, 1, blocks, bs, hkv, d)
+    dev = pool.device()
+    q = torch.from_numpy(rng.standard_normal((sum(q_lens), hq, d))).to(torch.bfloat16).cuda()
+    cu = torch.tensor([0, *np.cumsum(q_lens)], dtype=torch.int32, device="cuda")
+    c, b = torch.tensor(ctx, dtype=torch.int32, device="cuda"), bt.cuda()
+
+    def call(out=None):
+        return ops.paged_prefill_fp8(q, *dev, 0, b, cu, c, max(q_lens), bs, d ** -0.5, out=out)
+
+    want = call()
+    outs = [torch.empty_like(q) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    for out, stream in zip(outs, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(out)
+        graphs.append(graph)
+        for _ in range(63):
+            call()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert torch.equal(out, want)
