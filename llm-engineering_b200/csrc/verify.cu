@@ -116,6 +116,91 @@ __device__ __forceinline__ double piece_sum(const T* p, const T* q, int drop, in
   return warp_sum(s);
 }
 
+// kLoads * 16 bytes of both rows from entry a on, kept as they come.
+template <typename T, int kLoads>
+struct Run {
+  static constexpr int kPer = 16 / sizeof(T);
+  static constexpr int kEntries = kLoads * kPer;
+  uint4 u[kLoads], w[kLoads];
+
+  // Zeros from w1 on; 16-byte loads where both rows start on a 16-byte boundary (a is a multiple
+  // of as much).
+  __device__ __forceinline__ void load(const T* p, const T* q, int a, int w1) {
+    const bool wide = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0;
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+      const int at = a + c * kPer;
+      u[c] = w[c] = make_uint4(0, 0, 0, 0);
+      if (wide && at + kPer <= w1) {
+        u[c] = __ldg(reinterpret_cast<const uint4*>(p + at));
+        if (q != nullptr) w[c] = __ldg(reinterpret_cast<const uint4*>(q + at));
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          if (at + k < w1) {
+            reinterpret_cast<T*>(&u[c])[k] = p[at + k];
+            if (q != nullptr) reinterpret_cast<T*>(&w[c])[k] = q[at + k];
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ double residual(int e) const {  // of entry a + e (not the dropped one)
+    return positive((double)to_f32<T>(reinterpret_cast<const T*>(&u[e / kPer])[e % kPer]) -
+                    (double)to_f32<T>(reinterpret_cast<const T*>(&w[e / kPer])[e % kPer]));
+  }
+};
+
+// The first entry of [w0, w1) at which the running sum, `at` before w0, passes goal goes to *pick
+// (which no later entry then replaces), the last one with anything to *tail. The piece is read once,
+// a contiguous run per thread and round that stays in registers between the scan and the search.
+template <typename T, int kLoads>
+__device__ __forceinline__ void find_crossing(const T* prow, const T* qrow, int drop, int w0, int w1, double at,
+                                              double goal, bool crossing, double* scan, int* pick, int* tail) {
+  constexpr int kNone = 0x7fffffff;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r0 = w0; r0 < w1; r0 += kThreads * Run<T, kLoads>::kEntries) {
+    const int a = r0 + (int)threadIdx.x * Run<T, kLoads>::kEntries;
+    Run<T, kLoads> x;
+    x.load(prow, qrow, a, w1);
+    double mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < Run<T, kLoads>::kEntries; ++e) mine += a + e == drop ? 0.0 : x.residual(e);
+    double incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    double before = at;
+    for (int k = 0; k < kWarps; ++k) {
+      if (k < warp) before += scan[k];
+      at += scan[k];
+    }
+    before += incl - mine;
+    int first = kNone, last_one = -1;
+#pragma unroll
+    for (int e = 0; e < Run<T, kLoads>::kEntries; ++e) {
+      const double r = a + e == drop ? 0.0 : x.residual(e);
+      before += r;
+      if (r > 0.0) {
+        last_one = a + e;
+        if (crossing && before > goal) first = min(first, a + e);
+      }
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    last_one = __reduce_max_sync(0xffffffffu, last_one);
+    if (lane == 0) {
+      atomicMin(pick, first);
+      atomicMax(tail, last_one);
+    }
+    __syncthreads();
+    if (*pick < kNone) return;
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) verify_drafts(const VerifyParams p) {
   __shared__ Row row;
@@ -174,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_drafts(const VerifyParams 
     }
   }
   if (threadIdx.x == 0) {
-    pick = p.vocab;
+    pick = 0x7fffffff;
     tail = -1;
   }
   __syncthreads();
@@ -248,37 +333,16 @@ __global__ void __launch_bounds__(kThreads, 2) verify_drafts(const VerifyParams 
   }
   const bool crossing = ow >= 0;
   if (!crossing) ow = lw;
-  // the piece again, a contiguous run per thread
+  // The piece again. One load of each row per thread where two rounds of that cover it: long runs
+  // of few threads take longer than a round saves (one sequence 10.3 us with three, 8.7 with one;
+  // 256 of them, whose pieces are longer, 47 with three).
   const int w0 = min(p.vocab, (rank * kWarps + ow) * len), w1 = min(p.vocab, w0 + len);
-  const int per = (len + kThreads - 1) / kThreads;
-  const int a = min(w1, w0 + (int)threadIdx.x * per), b = min(w1, a + per);
-  double mine = 0.0;
-  for (int v = a; v < b; ++v) mine += residual<T>(prow, qrow, drop, v);
-  double incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 31) scan[warp] = incl;
-  __syncthreads();
-  double at = start;
-  for (int w = 0; w < warp; ++w) at += scan[w];
-  at += incl - mine;
-  for (int v = a; v < b; ++v) {
-    const double x = residual<T>(prow, qrow, drop, v);
-    at += x;
-    if (x > 0.0) {
-      atomicMax(&tail, v);
-      if (crossing && at > goal) {
-        atomicMin(&pick, v);
-        break;
-      }
-    }
-  }
-  __syncthreads();
+  if (len <= 2 * kThreads * Run<T, 1>::kEntries)
+    find_crossing<T, 1>(prow, qrow, drop, w0, w1, start, goal, crossing, scan, &pick, &tail);
+  else
+    find_crossing<T, 3>(prow, qrow, drop, w0, w1, start, goal, crossing, scan, &pick, &tail);
   if (threadIdx.x == 0)
-    p.out[(int64_t)seq * p.out_row + row.n] = pick < p.vocab ? pick : tail;
+    p.out[(int64_t)seq * p.out_row + row.n] = pick != 0x7fffffff ? pick : tail;
 }
 
 // Greedy form: the target rows are given by their arg-max ids; a draft stands while it equals
@@ -349,8 +413,8 @@ extern "C" int b2p_verify_drafts(const void* target_probs, int64_t target_row_st
   p.err = err_flag;
   cudaLaunchConfig_t cfg = {};
   // CTAs per sequence: as many as fill the GPU with one wave (two CTAs per SM). More only repeat
-  // the search for the first rejected draft: 256 sequences over 151,936 entries take 48.7 us with
-  // one CTA each, 52 with two, 76 with eight; one sequence takes 23.6, 15.4 and 8.8 us.
+  // the search for the first rejected draft: 256 sequences over 151,936 entries took 48.6 us with
+  // one CTA each, 52 with two, 76 with eight; one sequence 21.7, 14.2 and 8.3 us.
   int ranks = kMostRanks;
   while (ranks > 1 && (int64_t)num_seqs * ranks > 2LL * b2p_host::sm_count()) ranks /= 2;
   cfg.gridDim = dim3((unsigned)(num_seqs * ranks));
