@@ -11,11 +11,17 @@
 // The work is pure streaming: every new row is read once, its codes are written once. A warp holds
 // its rows in registers between the two (16 rows of 128 take 8 16-byte pieces a lane); where they
 // do not fit it reads them again, from L2.
+#include <type_traits>
+
 #include "fp8.cuh"
 
 namespace {
 
 using namespace b2p;
+
+constexpr int kWriteThreads = 128;
+template <typename T>
+constexpr int kWriteCtas = sizeof(T) == 4 ? 4 : 6;  // CTAs of the write per SM
 
 struct WriteFp8Params {
   const uint8_t* k;
@@ -30,7 +36,9 @@ struct WriteFp8Params {
   const int32_t* cu;
   const int32_t* ctx;
   int64_t num_rows, num_blocks;
-  int num_seqs, max_q_len, touched, hkv, d, block_size;
+  int num_seqs, max_q_len, hkv, d, block_size;
+  unsigned touched;  // blocks that a sequence may touch
+  int block_warps;
   bool vec;   // every row of keys and values starts on a 16-byte boundary
   bool seek;  // units are the touched blocks alone, found by a scan of the lengths
   int32_t* err;
@@ -84,15 +92,62 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, f
   return lo | (uint32_t)hi << 16;
 }
 
+// What turns a block's values into codes: inv = 2^-e. Where `packed`, 16-bit values are multiplied in
+// pairs in their own type: a power of two leaves their bits alone except below the normal range
+// (f16: 2^-14), where the code is zero either way (e4m3 rounds to zero up to 2^-10).
+struct Coder {
+  float inv;
+  bool clamp;     // some value is above kFp8Saturate
+  bool packed;
+  uint32_t inv2;  // a pair of inv in the values' type
+};
+
 template <typename T>
-__device__ __forceinline__ uint2 codes8(const Piece<T>& p, float inv, bool clamp) {
+__device__ __forceinline__ Coder coder_of(float s, float top) {
+  Coder c;
+  c.inv = 1.f / s;
+  c.clamp = top > kFp8Saturate;
+  c.inv2 = pack2<T>(c.inv, c.inv);
+  // f16 holds 2^-24 to 2^15; a scale kept from rows that another program wrote may be no power of two
+  c.packed = !c.clamp && (__float_as_uint(c.inv) & 0x7fffffu) == 0 &&
+             (std::is_same<T, __nv_bfloat16>::value || (c.inv <= 0x1p15f && c.inv >= 0x1p-24f));
+  return c;
+}
+template <>
+__device__ __forceinline__ Coder coder_of<float>(float s, float top) {
+  return Coder{1.f / s, top > kFp8Saturate, false, 0u};
+}
+
+__device__ __forceinline__ uint16_t codes2_packed(uint32_t w, uint32_t inv2, __half) {
+  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&inv2));
+  return __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(y), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint16_t codes2_packed(uint32_t w, uint32_t inv2, __nv_bfloat16) {
+  const __nv_bfloat162 y =
+      __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&inv2));
+  const uint32_t b = *reinterpret_cast<const uint32_t*>(&y);
+  return __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)),
+                                  __NV_SATFINITE, __NV_E4M3);
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const Piece<T>& p, const Coder& c) {
+  if constexpr (sizeof(T) == 2) {
+    if (c.packed) {
+      const uint32_t in[4] = {p.w.x, p.w.y, p.w.z, p.w.w};
+      uint32_t two[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) two[i] = codes2_packed(in[i], c.inv2, T());
+      return make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+    }
+  }
   float x[8];
   p.values(x);
-  if (clamp) {
+  if (c.clamp) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -kFp8Saturate), kFp8Saturate);
   }
-  return make_uint2(codes4(x[0], x[1], x[2], x[3], inv), codes4(x[4], x[5], x[6], x[7], inv));
+  return make_uint2(codes4(x[0], x[1], x[2], x[3], c.inv), codes4(x[4], x[5], x[6], x[7], c.inv));
 }
 
 // The block's scale from the largest magnitude of its new rows; NaN where a row is not finite or
@@ -119,62 +174,95 @@ __device__ __forceinline__ void rescale(uint8_t* dst, int64_t row_bytes, int d, 
 
 constexpr int kHold = 8;  // pieces of eight elements that a lane keeps
 
-// One warp: n rows of one head into slots off0 .. off0 + n - 1 of a block, by 16-byte pieces. kD:
-// the head dim where it is known, which spares the divisions by a row's pieces (32 prompts written
-// and read back: 40.7 us against 45.5), 0 otherwise.
+// n rows of one head for slots off0 .. off0 + n - 1 of a block.
+template <typename T>
+struct Target {
+  const T* src;
+  uint8_t* dst;  // slot 0 of the block
+  float* scale;
+  int64_t tok;
+  int off0, n;
+};
+
+// One warp writes a target, by 16-byte pieces: load() sends for the rows, finish() does the rest.
+// kD: the head dim where it is known and a row's pieces divide the warp's lanes, 0 otherwise. Then
+// a lane's pieces are one column of every 256 / kD-th row, and neither divisions nor bounds on
+// pieces are left.
 template <typename T, int kD>
-__device__ void write_block_vec(const T* src, int64_t tok, uint8_t* dst, int64_t row_bytes,
-                                float* scale, int head_dim, int off0, int n, int lane) {
-  const int d = kD != 0 ? kD : head_dim;
-  const int per_row = d / 8, total = n * per_row;
-  const bool keep = off0 > 0;
-  const float old = keep ? *scale : 0.f;  // one address for the warp
-  uint32_t m = 0;
+struct BlockWriter {
+  static constexpr int kStep = kD != 0 ? 256 / kD : 1;  // rows from one of a lane's pieces to its next
+  int lane, per_row, row0, col;
+  int64_t row_bytes;
   Piece<T> held[kHold];
-  const bool fits = total <= 32 * kHold;
-  auto at = [&](int i) { return src + (int64_t)(i / per_row) * tok + (i % per_row) * 8; };
-  if (fits) {
-#pragma unroll
-    for (int k = 0; k < kHold; ++k)
-      if (lane + 32 * k < total) held[k].load(at(lane + 32 * k));
-#pragma unroll
-    for (int k = 0; k < kHold; ++k)
-      if (lane + 32 * k < total) held[k].max_bits(m);
-  } else {
-    for (int i = lane; i < total; i += 32) {
-      held[0].load(at(i));
-      held[0].max_bits(m);
-    }
+  float old;
+
+  __device__ __forceinline__ BlockWriter(int head_dim, int64_t row_bytes)
+      : lane(threadIdx.x & 31), per_row((kD != 0 ? kD : head_dim) / 8), row0(kD != 0 ? lane / per_row : 0),
+        col(kD != 0 ? lane % per_row : 0), row_bytes(row_bytes) {}
+  __device__ __forceinline__ bool fits(const Target<T>& t) const { return t.n * per_row <= 32 * kHold; }
+  __device__ __forceinline__ bool have(const Target<T>& t, int k) const {
+    return kD != 0 ? row0 + k * kStep < t.n : lane + 32 * k < t.n * per_row;
   }
-  const float amax = Piece<T>::magnitude(m);
-  // bits again: __reduce_max_sync orders NaN and infinities above every number
-  const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-  const float s = new_scale(top, old, keep);
-  const bool bad = s != s;
-  if (keep && !bad && s != old) rescale(dst, row_bytes, d, off0, old / s, lane);
-  const float inv = bad ? 0.f : 1.f / s;
-  const bool clamp = top > kFp8Saturate;
-  auto put = [&](int i, const Piece<T>& p) {
-    const uint2 c = bad ? make_uint2(0u, 0u) : codes8<T>(p, inv, clamp);
-    reinterpret_cast<uint2*>(dst + (int64_t)(off0 + i / per_row) * row_bytes)[i % per_row] = c;
-  };
-  if (fits) {
+  __device__ __forceinline__ const T* from(const Target<T>& t, int k) const {
+    if (kD != 0) return t.src + (row0 + k * kStep) * t.tok + col * 8;
+    const int i = lane + 32 * k;
+    return t.src + (i / per_row) * t.tok + (i % per_row) * 8;
+  }
+  __device__ __forceinline__ uint2* to(const Target<T>& t, int k) const {
+    if (kD != 0) return reinterpret_cast<uint2*>(t.dst + (t.off0 + row0 + k * kStep) * row_bytes) + col;
+    const int i = lane + 32 * k;
+    return reinterpret_cast<uint2*>(t.dst + (t.off0 + i / per_row) * row_bytes) + i % per_row;
+  }
+  __device__ __forceinline__ void load(const Target<T>& t) {
+    old = t.off0 > 0 ? *t.scale : 0.f;  // one address for the warp
+    if (!fits(t)) return;
 #pragma unroll
     for (int k = 0; k < kHold; ++k)
-      if (lane + 32 * k < total) put(lane + 32 * k, held[k]);
-  } else {
-    for (int i = lane; i < total; i += 32) {
-      held[0].load(at(i));
-      put(i, held[0]);
-    }
+      if (have(t, k)) held[k].load(from(t, k));
   }
-  if (lane == 0) *scale = s;
-}
+  __device__ __forceinline__ void finish(const Target<T>& t) {
+    const bool keep = t.off0 > 0, whole = fits(t);
+    uint32_t m = 0;
+    if (whole) {
+#pragma unroll
+      for (int k = 0; k < kHold; ++k)
+        if (have(t, k)) held[k].max_bits(m);
+    } else {
+      for (int k = 0; have(t, k); ++k) {
+        held[0].load(from(t, k));
+        held[0].max_bits(m);
+      }
+    }
+    const float amax = Piece<T>::magnitude(m);
+    // bits again: __reduce_max_sync orders NaN and infinities above every number
+    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+    const float s = new_scale(top, old, keep);
+    const bool bad = s != s;
+    if (keep && !bad && s != old) rescale(t.dst, row_bytes, per_row * 8, t.off0, old / s, lane);
+    const Coder coder = coder_of<T>(s, top);
+    auto put = [&](int k, const Piece<T>& x) { *to(t, k) = bad ? make_uint2(0u, 0u) : codes8<T>(x, coder); };
+    if (whole) {
+#pragma unroll
+      for (int k = 0; k < kHold; ++k)
+        if (have(t, k)) put(k, held[k]);
+    } else {
+      for (int k = 0; have(t, k); ++k) {
+        held[0].load(from(t, k));
+        put(k, held[0]);
+      }
+    }
+    if (lane == 0) *t.scale = s;
+  }
+};
 
 // The same by single elements, for rows that are not 16-byte aligned.
 template <typename T>
-__device__ void write_block_elem(const T* src, int64_t tok, uint8_t* dst, int64_t row_bytes,
-                                 float* scale, int d, int off0, int n, int lane) {
+__device__ __noinline__ void write_block_elem(const Target<T>& t, int64_t row_bytes, int d, int lane) {
+  const T* src = t.src;
+  uint8_t* dst = t.dst;
+  float* scale = t.scale;
+  const int64_t tok = t.tok;
+  const int off0 = t.off0, n = t.n;
   const bool keep = off0 > 0;
   const float old = keep ? *scale : 0.f;
   uint32_t m = 0;
@@ -212,70 +300,122 @@ __device__ __forceinline__ int touched_blocks(const Append& a, int block_size) {
   return a.qlen <= 0 ? 0 : (a.start + a.qlen - 1) / block_size - a.start / block_size + 1;
 }
 
-// A unit is (sequence, touched block, head, K or V), one per warp and round.
+// Where a sequence's new rows meet a block: rows row .. row + n - 1 go to its slots off0 ...
+struct Touched {
+  int64_t row;
+  int32_t block;
+  int off0, n;  // n 0: nothing to do here
+};
+
+// Touched block u of the batch; false past the last one.
+__device__ __forceinline__ bool find_touched(const WriteFp8Params& p, unsigned u, Touched& t) {
+  const int lane = threadIdx.x & 31;
+  int seq, j;
+  if (p.seek) {  // the sequence that holds it, 32 sequences at a time
+    int64_t want = u;
+    seq = -1;
+    j = 0;
+    for (int base = 0; base < p.num_seqs && seq < 0; base += 32) {
+      const int n = base + lane < p.num_seqs ? touched_blocks(append_of(p, base + lane), p.block_size) : 0;
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, incl > want);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        seq = base + src;
+        j = (int)(want - __shfl_sync(0xffffffffu, incl - n, src));
+      } else {
+        want -= __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    if (seq < 0) return false;
+  } else {
+    if (u >= (unsigned)p.num_seqs * p.touched) return false;
+    seq = u / p.touched;
+    j = u - seq * p.touched;
+  }
+  t.n = 0;
+  const Append a = append_of(p, seq);
+  if (a.qlen <= 0) return true;
+  const int ctx = a.start + a.qlen;
+  const int b = a.start / p.block_size + j;
+  const int lo = max(a.start, b * p.block_size);
+  const int hi = (int)min((int64_t)ctx, (int64_t)(b + 1) * p.block_size);
+  if (lo >= hi) return true;
+  t.block = b < p.bt_stride ? __ldg(p.block_tables + (int64_t)seq * p.bt_stride + b) : -1;
+  if (t.block < 0 || t.block >= p.num_blocks) {
+    if (lane == 0) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
+    return true;
+  }
+  t.row = a.q0 + (lo - a.start);
+  t.off0 = lo - b * p.block_size;
+  t.n = hi - lo;
+  return true;
+}
+
+// p.block_warps warps of a CTA share a touched block; a warp takes every so many of its (head, K or
+// V) targets, then those of a later block. While a target's rows are on their way the warp looks
+// for the next one: 53,400 f16 rows of 2 x 128 in 19.6 us against 22.5 with a search per target
+// and nothing in flight meanwhile (bytes alone: 12.5 us). Six CTAs per SM; with eight the rows no
+// longer fit the registers (24.6 us), with four that hold two targets each 22.0.
 template <typename T, int kD>
-__global__ void __launch_bounds__(128) kv_write_fp8_rows(const WriteFp8Params p) {
+__global__ void __launch_bounds__(kWriteThreads, kWriteCtas<T>) kv_write_fp8_rows(const WriteFp8Params p) {
   // The attention that follows may start its look at lengths and tables, which this kernel does
   // not write, while it runs; it waits for this grid's end before it touches the pool.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int per_block = 2 * p.hkv;
-  const int64_t per_seq = (int64_t)p.touched * per_block;
-  for (int64_t u = blockIdx.x * 4ll + (threadIdx.x >> 5);; u += gridDim.x * 4ll) {
-    int seq, j;
-    const int r = (int)(u % per_block), h = r >> 1;
-    if (p.seek) {
-      // the sequence that holds touched block u / per_block, 32 sequences at a time
-      int64_t want = u / per_block;
-      seq = -1;
-      j = 0;
-      for (int base = 0; base < p.num_seqs && seq < 0; base += 32) {
-        const int n = base + lane < p.num_seqs ? touched_blocks(append_of(p, base + lane), p.block_size) : 0;
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, incl > want);
-        if (hit) {
-          const int src = __ffs(hit) - 1;
-          seq = base + src;
-          j = (int)(want - __shfl_sync(0xffffffffu, incl - n, src));
-        } else {
-          want -= __shfl_sync(0xffffffffu, incl, 31);
-        }
-      }
-      if (seq < 0) return;  // past the last touched block
-    } else {
-      if (u >= per_seq * p.num_seqs) return;
-      seq = (int)(u / per_seq);
-      j = (int)(u - seq * per_seq) / per_block;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row_bytes = (int64_t)p.hkv * p.d;
+  const unsigned per_cta = kWriteThreads / 32 / p.block_warps;
+  const unsigned stride = gridDim.x * per_cta;
+  unsigned u = blockIdx.x * per_cta + warp / p.block_warps;
+  const int first = warp % p.block_warps;
+  int c = first;
+  Touched at;
+  bool more = find_touched(p, u, at);
+  auto settle = [&]() {  // on to a block with something to do
+    while (more && at.n == 0) {
+      u += stride;
+      more = find_touched(p, u, at);
     }
-    const Append a = append_of(p, seq);
-    if (a.qlen <= 0) continue;
-    const bool is_v = r & 1;
-    const int ctx = a.start + a.qlen;
-    const int b = a.start / p.block_size + j;
-    const int lo = max(a.start, b * p.block_size);
-    const int hi = (int)min((int64_t)ctx, (int64_t)(b + 1) * p.block_size);
-    if (lo >= hi) continue;
-    const int32_t blk = b < p.bt_stride ? __ldg(p.block_tables + (int64_t)seq * p.bt_stride + b) : -1;
-    if (blk < 0 || blk >= p.num_blocks) {
-      if (lane == 0) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
-      continue;
+  };
+  settle();
+  auto target = [&]() {
+    Target<T> t;
+    const int h = c >> 1;
+    const bool is_v = c & 1;
+    t.tok = is_v ? p.v_tok : p.k_tok;
+    t.src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + at.row * t.tok + h * (is_v ? p.v_head : p.k_head);
+    t.dst = (is_v ? p.v_cache : p.k_cache) + (int64_t)at.block * p.block_size * row_bytes + (int64_t)h * p.d;
+    t.scale = (is_v ? p.v_scales : p.k_scales) + (int64_t)at.block * p.hkv + h;
+    t.off0 = at.off0;
+    t.n = at.n;
+    return t;
+  };
+  auto advance = [&]() {
+    c += p.block_warps;
+    if (c < 2 * p.hkv) return;
+    c = first;
+    u += stride;
+    more = find_touched(p, u, at);
+    settle();
+  };
+  if (p.vec) {
+    BlockWriter<T, kD> writer(p.d, row_bytes);
+    while (more) {
+      const Target<T> t = target();
+      writer.load(t);
+      advance();
+      writer.finish(t);
     }
-    const int64_t row_bytes = (int64_t)p.hkv * p.d;
-    uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + (int64_t)blk * p.block_size * row_bytes + (int64_t)h * p.d;
-    float* scale = (is_v ? p.v_scales : p.k_scales) + (int64_t)blk * p.hkv + h;
-    const int64_t row = a.q0 + (lo - a.start);
-    const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) +
-                   (is_v ? row * p.v_tok + h * p.v_head : row * p.k_tok + h * p.k_head);
-    const int off0 = lo - b * p.block_size;
-    if (p.vec)
-      write_block_vec<T, kD>(src, is_v ? p.v_tok : p.k_tok, dst, row_bytes, scale, p.d, off0, hi - lo, lane);
-    else
-      write_block_elem<T>(src, is_v ? p.v_tok : p.k_tok, dst, row_bytes, scale, p.d, off0, hi - lo, lane);
+  } else {
+    while (more) {
+      write_block_elem<T>(target(), row_bytes, p.d, lane);
+      advance();
+    }
   }
 }
 
@@ -405,7 +545,7 @@ extern "C" int b2p_kv_write_fp8(const void* keys, int64_t k_tok_stride, int64_t 
   p.num_seqs = num_seqs;
   p.num_rows = num_rows;
   p.max_q_len = max_q_len;
-  p.touched = (int)(((int64_t)max_q_len + block_size - 2) / block_size + 1);
+  p.touched = (unsigned)(((int64_t)max_q_len + block_size - 2) / block_size + 1);
   p.hkv = num_kv_heads;
   p.d = head_dim;
   p.block_size = block_size;
@@ -415,20 +555,24 @@ extern "C" int b2p_kv_write_fp8(const void* keys, int64_t k_tok_stride, int64_t 
             (uintptr_t)(k_head_stride * es) | (uintptr_t)(v_tok_stride * es) | (uintptr_t)(v_head_stride * es)) & 15u) == 0;
   // Units by (sequence, block number) where every sequence touches about as many blocks as the
   // longest may; in a batch of unlike lengths most of those are empty (32 prompts of 64 to 8192
-  // tokens: 4 of 5, 46 us), and the touched ones are found by a scan instead.
+  // tokens: 4 of 5), and the touched ones are found by a scan instead.
   const int64_t direct = (int64_t)num_seqs * p.touched;
   const int64_t bound = num_rows / block_size + 2ll * num_seqs;
   p.seek = direct > 2 * bound;
-  const int64_t warps = (p.seek ? bound : direct) * num_kv_heads * 2;
-  const int64_t most = (int64_t)b2p_host::sm_count() * 16;
-  const unsigned grid = (unsigned)((warps + 3) / 4 < most ? (warps + 3) / 4 : most);
+  const int64_t units = p.seek ? bound : direct;
+  if (units > 0x3fffffffLL) return B2P_EUNSUPPORTED;
+  p.block_warps = num_kv_heads == 1 ? 2 : 4;
+  const int per_cta = kWriteThreads / 32 / p.block_warps;
+  const int64_t ctas = (units + per_cta - 1) / per_cta;
+  const int64_t most = (int64_t)b2p_host::sm_count() * (dtype == B2P_F32 ? kWriteCtas<float> : kWriteCtas<__half>);
+  const unsigned grid = (unsigned)(ctas < most ? ctas : most);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int kind = head_dim == 128 ? 2 : head_dim == 64 ? 1 : 0;
   void (*const fns[3][3])(WriteFp8Params) = {
       {kv_write_fp8_rows<__nv_bfloat16, 0>, kv_write_fp8_rows<__nv_bfloat16, 64>, kv_write_fp8_rows<__nv_bfloat16, 128>},
       {kv_write_fp8_rows<__half, 0>, kv_write_fp8_rows<__half, 64>, kv_write_fp8_rows<__half, 128>},
       {kv_write_fp8_rows<float, 0>, kv_write_fp8_rows<float, 64>, kv_write_fp8_rows<float, 128>}};
-  fns[dtype][kind]<<<grid, 128, 0, s>>>(p);
+  fns[dtype][kind]<<<grid, kWriteThreads, 0, s>>>(p);
   return b2p_host::check_launch();
 }
 

@@ -561,3 +561,41 @@ def test_captured_prompts_replayed_side_by_side(ops):
         torch.cuda.synchronize()
         for out in outs:
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("hkv,d,dtype", [(3, 64, torch.bfloat16), (1, 128, torch.float16), (5, 32, torch.float32)])
+@pytest.mark.parametrize("even", [False, True])
+def test_write_of_more_blocks_than_run_at_once(ops, hkv, d, dtype, even):
+    """Warps that take many blocks in turn, with sequences that bring nothing or do not fit between them."""
+    bs, n = 16, 60
+    rng = np.random.default_rng(hkv + d)
+    q_lens = [470] * n if even else [int(x) for x in rng.choice([0, 1, 15, 40, 700, 1100], n)]
+    past = [int(x) for x in rng.integers(0, 40, n)]
+    ctx = [a + b for a, b in zip(past, q_lens)]
+    tables, bt, blocks = tables_for(rng, ctx, bs)
+    pool = Pool(rng, 1, blocks, bs, hkv, d)
+    new = [torch.from_numpy(rng.standard_normal((sum(q_lens), hkv, d)) * s).to(dtype) for s in (3.0, 0.01)]
+    cu = [0, *np.cumsum(q_lens)]
+    dev = pool.device()
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    bad = int(np.argmax(q_lens))  # its context is one short of its rows: refused
+    told = list(ctx)
+    told[bad] = q_lens[bad] - 1
+    ops.kv_write_fp8(*dev, 0, bt.cuda(), torch.tensor(cu, dtype=torch.int32, device="cuda"),
+                     torch.tensor(told, dtype=torch.int32, device="cuda"), max(q_lens), bs, new[0].cuda(),
+                     new[1].cuda(), err_flag=err)
+    assert err.item() == 8
+    fits = [i for i in range(n) if i != bad]
+    rows = np.concatenate([np.arange(cu[i], cu[i + 1]) for i in fits])
+    for codes, scales, x in ((pool.k, pool.ks, new[0]), (pool.v, pool.vs, new[1])):
+        ref.write(codes[0].numpy(), scales[0].numpy(), bs, [tables[i] for i in fits], [q_lens[i] for i in fits],
+                  [ctx[i] for i in fits], x.double().numpy()[rows])
+    used = np.zeros(blocks * bs, dtype=bool)  # slots of the touched blocks behind the context are free
+    for i in fits:
+        if q_lens[i]:
+            last = tables[i][(ctx[i] - 1) // bs]
+            used[last * bs + (ctx[i] - 1) % bs + 1:(last + 1) * bs] = True
+    for got, want in zip(dev[:2], (pool.k, pool.v)):
+        assert torch.equal(got.view(torch.uint8).cpu()[0][~used], want[0][~used])
+    for got, want in zip(dev[2:], (pool.ks, pool.vs)):
+        assert torch.equal(got.double().cpu(), want)
