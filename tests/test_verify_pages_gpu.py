@@ -230,3 +230,33 @@ def test_compact_flags_bad_tables(ops):
     assert bt.tolist() == [[2, 12, 3], [-1, 0, 1]]
     for t, b in zip(p, before):
         assert torch.equal(t[:, 32:48], b[:, 144:160])
+
+
+@pytest.mark.parametrize("blocks,width", [(3000, 1170), (3000, 1171), (2049, 4000), (40, 9000)])
+def test_compact_wide_tables(ops, blocks, width):
+    """Tables of up to and over what one CTA looks through, pools that end inside a word of bits."""
+    n, bs = 7, 16
+    rng = np.random.default_rng(width)
+    p = pool(3, torch.bfloat16, 1, blocks, bs, 1, 8)
+    ids = rng.permutation(blocks)[:blocks * 3 // 5].tolist()
+    cuts = sorted(rng.integers(0, len(ids) + 1, n - 1).tolist())
+    tables = [ids[a:b][:width] for a, b in zip([0, *cuts], [*cuts, len(ids)])]
+    ctx = [max(0, len(t) * bs - int(rng.integers(0, bs))) for t in tables]
+    bt = torch.from_numpy(rng.integers(0, blocks, (n, width))).to(torch.int32)  # stale ids behind the context
+    for i, t in enumerate(tables):
+        bt[i, :len(t)] = torch.tensor(t, dtype=torch.int32)
+    moves, new, live = ref.compact(tables, ctx, bs, blocks)
+    want = [raw(t, bs).clone() for t in p[:2]]
+    for s, t in moves:
+        for w in want:
+            w[:, t] = w[:, s]
+    want_bt = bt.clone()
+    for i, c in enumerate(ctx):
+        used = -(-c // bs)
+        want_bt[i, :used] = torch.tensor(new, dtype=torch.int32)[bt[i, :used].long()]
+    err, dev_bt = i32([0]), bt.cuda()
+    got_new, got_live = ops.compact_blocks(p[0], p[1], dev_bt, i32(ctx), bs, err_flag=err)
+    assert err.item() == 0 and got_live.tolist() == [live] and got_new.tolist() == new
+    assert torch.equal(dev_bt.cpu(), want_bt)
+    for t, w in zip(p, want):
+        assert torch.equal(raw(t, bs), w)
