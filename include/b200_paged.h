@@ -344,6 +344,8 @@ B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, cons
 B2P_API size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total_q,
                  int64_t table_width, int num_q_heads, int num_kv_heads, int head_dim, int block_size, int max_q_len,
                  int dtype);
+/* Calls with max_q_len * num_q_heads / num_kv_heads up to this need no scratch. */
+B2P_API int b2p_paged_fp8_row_columns(void);
 B2P_API size_t b2p_paged_fp8_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads,
                                             int head_dim, int max_q_len);
 B2P_API int b2p_paged_decode_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,

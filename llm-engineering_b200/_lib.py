@@ -47,6 +47,7 @@ EXPORTED_SYMBOLS = (
     "b2p_lm_head_argmax",
     "b2p_kv_write_fp8",
     "b2p_kv_read_fp8",
+    "b2p_paged_fp8_row_columns",
     "b2p_paged_fp8_workspace_size",
     "b2p_paged_decode_fp8",
     "b2p_paged_prefill_fp8_scratch_size",
@@ -117,6 +118,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_p, _p, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p],
     ),
+    "b2p_paged_fp8_row_columns": (_i32, []),
     "b2p_paged_fp8_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "b2p_paged_decode_fp8": (
         _i32,

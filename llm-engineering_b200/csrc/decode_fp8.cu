@@ -1101,6 +1101,8 @@ bool b2p_rows_fp8_takes(int group, int head_dim, int block_size, int dtype, int 
          select_fp8_plan<__half>(head_dim, group * max_q_len, pl);
 }
 
+extern "C" int b2p_paged_fp8_row_columns(void) { return kRowColumns; }
+
 size_t b2p_rows_fp8_workspace(int num_seqs, int num_kv_heads) {
   // a sequence has at most kRowColumns / 8 column groups (8 columns being the least a pass takes)
   const size_t counters = (size_t)num_kv_heads * num_seqs * (kRowColumns / 8) * 4;

@@ -8,6 +8,8 @@ wrong device or a missing library raises instead of falling back.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -383,7 +385,8 @@ FP8_DTYPE = torch.float8_e4m3fn
 
 
 # The current stream's handle and the current device's index without torch.cuda's wrappers: the
-# calls below take a few microseconds on the host, of which those two would be one.
+# calls below take a few microseconds on the host, of which those two would be one. For the same
+# reason outputs come from torch.empty_strided, in two thirds of torch.empty's time.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -419,7 +422,8 @@ def _vector(index: int, name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
     if t.dtype is not dtype or not t.is_contiguous():
         _require_cuda(name, t)
         raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor")
-    _on(index, name, t)
+    if t.get_device() != index:
+        _on(index, name, t)
 
 
 def _err_flag(index: int, err_flag: torch.Tensor | None) -> int | None:
@@ -432,7 +436,9 @@ def _err_flag(index: int, err_flag: torch.Tensor | None) -> int | None:
 def _check_fp8_pool(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: torch.Tensor,
                     value_scales: torch.Tensor, block_size: int) -> tuple[int, torch.Size]:
     """(device index, pool shape) of a valid 8-bit pool."""
-    index = _index_of("key_cache", key_cache)
+    index = key_cache.get_device()
+    if index < 0:
+        _require_cuda("key_cache", key_cache)
     shape = key_cache.shape
     if value_cache.shape != shape or len(shape) != 4:
         raise ValueError("key_cache/value_cache must both be [layers, slots, kv_heads, head_dim]")
@@ -440,12 +446,14 @@ def _check_fp8_pool(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scal
         raise ValueError(f"an 8-bit pool must be {FP8_DTYPE} (got {key_cache.dtype}, {value_cache.dtype})")
     if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
         raise ValueError("key_cache/value_cache must be contiguous")
-    _on(index, "value_cache", value_cache)
-    if block_size <= 0 or shape[1] % block_size:
+    layers, slots, hkv, _ = shape
+    if block_size <= 0 or slots % block_size:
         raise ValueError("the pool's slots must be a multiple of block_size")
-    want = (shape[0], shape[1] // block_size, shape[2])
+    want = (layers, slots // block_size, hkv)
     if key_scales.shape != want or value_scales.shape != want:
         raise ValueError(f"key_scales/value_scales must have shape {want}")
+    if value_cache.get_device() != index:
+        _on(index, "value_cache", value_cache)
     _vector(index, "key_scales", key_scales, torch.float32)
     _vector(index, "value_scales", value_scales, torch.float32)
     return index, shape
@@ -531,13 +539,19 @@ def kv_read_fp8(
     _vector(index, "slot_mapping", slot_mapping, torch.int32)
     code = dtype_code(dtype)
     n = slot_mapping.numel()
-    keys = torch.empty((n, hkv, d), dtype=dtype, device=key_cache.device)
+    keys = torch.empty_strided((n, hkv, d), (hkv * d, d, 1), dtype=dtype, device=key_cache.device)
     values = torch.empty_like(keys)
     _call("b2p_kv_read_fp8", index, key_cache.data_ptr(), value_cache.data_ptr(),
           key_scales.data_ptr(), value_scales.data_ptr(), slot_mapping.data_ptr(), n,
           keys.data_ptr(), values.data_ptr(), layer_index, layers, slots, hkv, d, block_size, code,
           _err_flag(index, err_flag))
     return keys, values
+
+
+@functools.cache
+def _row_columns() -> int:
+    """(row, query head of a KV head) pairs per sequence up to which a call needs no scratch."""
+    return int(_lib.load().b2p_paged_fp8_row_columns())
 
 
 def fp8_workspace_size(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
@@ -560,13 +574,15 @@ def _fp8_query(index: int, head_dim: int, q: torch.Tensor, out: torch.Tensor | N
     if q.dim() != 3 or q.shape[2] != head_dim:
         raise ValueError("q must be (rows, num_q_heads, head_dim) with the pool's head_dim")
     code = dtype_code(q.dtype)
+    qt, qh, qd = q.stride()
     if out is None:
+        if q.is_contiguous():
+            return code, torch.empty_like(q), qt, qh, q.shape[1] * head_dim, head_dim
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _on(index, "out", out)
         if out.shape != q.shape or out.dtype is not q.dtype:
             raise ValueError("out must have q's shape and dtype")
-    qt, qh, qd = q.stride()
     ot, oh, od = out.stride()
     if qd != 1 or od != 1:
         raise ValueError("q and out must have a contiguous head_dim")
@@ -649,9 +665,11 @@ def paged_prefill_fp8(
     _vector(index, "cu_seqlens_q", cu_seqlens_q, torch.int32)
     width = _check_tables(index, n, block_tables, context_lens)
     workspace = _fp8_workspace(index, workspace, n, hq, hkv, d, max_q_len)
-    size = _lib.load().b2p_paged_prefill_fp8_scratch_size(n, total_q, width, hq, hkv, d,
-                                                          block_size, max_q_len, code)
-    scratch = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    scratch, size = None, 0
+    if max_q_len * hq > _row_columns() * hkv:
+        size = _lib.load().b2p_paged_prefill_fp8_scratch_size(n, total_q, width, hq, hkv, d,
+                                                              block_size, max_q_len, code)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     _call("b2p_paged_prefill_fp8", index, q.data_ptr(), qt, qh, key_cache.data_ptr(),
           value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
           layers, slots, block_tables.data_ptr(), width, cu_seqlens_q.data_ptr(),
@@ -662,8 +680,9 @@ def paged_prefill_fp8(
 
 
 def _drafts_out(n: int, max_drafts: int, device: torch.device):
-    return (torch.empty((n, max_drafts + 1), dtype=torch.int64, device=device),
-            torch.empty(n, dtype=torch.int32, device=device))
+    row = max_drafts + 1
+    return (torch.empty_strided((n, row), (row, 1), dtype=torch.int64, device=device),
+            torch.empty_strided((n,), (1,), dtype=torch.int32, device=device))
 
 
 def _check_drafts(index: int, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor,
@@ -817,9 +836,9 @@ def compact_blocks(
     width = _check_tables(index, n, block_tables, context_lens)
     dev, blocks = key_cache.device, slots // block_size
     size = _lib.load().b2p_compact_blocks_workspace_size(blocks)
-    workspace = torch.empty(size, dtype=torch.uint8, device=dev)
-    new_ids = torch.empty(blocks, dtype=torch.int32, device=dev)
-    num_live = torch.empty(1, dtype=torch.int32, device=dev)
+    workspace = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=dev)
+    new_ids = torch.empty_strided((blocks,), (1,), dtype=torch.int32, device=dev)
+    num_live = torch.empty_strided((1,), (1,), dtype=torch.int32, device=dev)
     _call("b2p_compact_blocks", index, key_cache.data_ptr(), value_cache.data_ptr(),
           _ptr(key_scales), _ptr(value_scales), block_tables.data_ptr(), width, width, context_lens.data_ptr(), n, layers, slots, hkv, d,
           key_cache.element_size(), block_size, new_ids.data_ptr(), num_live.data_ptr(),
