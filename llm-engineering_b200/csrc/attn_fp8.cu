@@ -61,6 +61,7 @@ bool rows_fit(const void* q, int64_t q_tok, int64_t q_head, const void* kc, cons
 using namespace b2p;
 
 constexpr int kWidenThreads = 256;
+constexpr int kWidenLoads = 2;  // loads that a thread has in flight
 
 struct WidenParams {
   const uint8_t* codes[2];  // layer bases of K and V
@@ -70,6 +71,7 @@ struct WidenParams {
   const int32_t* block_tables;
   int64_t bt_stride;
   int width;
+  int parts, share;  // pieces of a block, rounds of the CTA's loads in each
   const int32_t* cu;
   const int32_t* ctx;
   int32_t* safe_cu;   // [num_seqs + 1] and [num_seqs]: the same within q's rows and the tables'
@@ -95,13 +97,17 @@ __device__ __forceinline__ int row_within(const WidenParams& p, int row) {
   return (int)min(max((int64_t)row, (int64_t)0), p.num_rows);
 }
 
-// A CTA takes the used blocks of all histories in turn (found by a scan of the lengths, 32
-// sequences at a time: with one CTA per table entry, most of a ragged batch's are empty, 35 us
+// A CTA takes pieces of the used blocks of all histories in turn (found by a scan of the lengths,
+// 32 sequences at a time: with one CTA per table entry, most of a ragged batch's are empty, 35 us
 // against 22 on 32 prompts) and writes their codes as 16-bit rows into the scratch block that the
-// scratch table gives them. Memory-bound: 1 byte read and 2 written per element.
+// // scratch table gives them. A piece is a whole block where there are many, else down to what the
+// CTA's threads have in flight at once (one sequence of 210 rows and 4 heads in blocks of 64: the call
+// takes 17.9 us, 22.5 with whole blocks). Memory-bound: 1 byte read and 2 written per element.
 template <typename T>
-__global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenParams p) {
+__global__ void __launch_bounds__(kWidenThreads, 8) widen_histories(const WidenParams p) {
   __shared__ int found[2];  // sequence (-1: no block left) and block number
+  // the tile kernel may set itself up meanwhile; it reads nothing before this grid has ended
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   if (blockIdx.x == 0 && threadIdx.x < 2) p.claims[threadIdx.x] = 0;
   for (int64_t i = blockIdx.x * (int64_t)kWidenThreads + threadIdx.x; i < p.num_lse;
@@ -125,10 +131,11 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
       reinterpret_cast<T*>(p.out)[row * p.o_tok + (int64_t)(r / p.d) * p.o_head + r % p.d] = from_f32<T>(0.f);
     }
   }
+  const int per_row = p.hkv * p.d / 16, per_head = p.d / 16;  // 16-code loads
   for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
     __syncthreads();  // the previous round has read `found`
     if (threadIdx.x < 32) {
-      int64_t want = unit;
+      int64_t want = unit / p.parts;
       int seq = -1, col = 0;
       for (int base = 0; base < p.num_seqs && seq < 0; base += 32) {
         const int s = base + lane;
@@ -157,39 +164,57 @@ __global__ void __launch_bounds__(kWidenThreads) widen_histories(const WidenPara
       }
     }
     __syncthreads();
-    const int seq = found[0], col = found[1];
+    const int seq = found[0], col = found[1], part = (int)(unit % p.parts);
     if (seq < 0) return;
     const int64_t w = (int64_t)seq * p.width + col;
-    if (threadIdx.x == 0) p.tables[w] = (int32_t)w;
     const int tokens = min(p.block_size, __ldg(p.ctx + seq) - col * p.block_size);
     const int32_t blk = __ldg(p.block_tables + (int64_t)seq * p.bt_stride + col);
     const bool have = blk >= 0 && blk < p.num_blocks;
-    if (!have && threadIdx.x == 0) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
-    const int per_row = p.hkv * p.d / 16, per_head = p.d / 16;  // 16-code pieces
-    for (int i = threadIdx.x; i < 2 * tokens * per_row; i += kWidenThreads) {
-      const bool is_v = i >= tokens * per_row;
-      const int at = is_v ? i - tokens * per_row : i;
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      float s = 0.f;
-      if (have) {
-        raw = __ldg(reinterpret_cast<const uint4*>(p.codes[is_v]) + (int64_t)blk * p.block_size * per_row + at);
-        const int64_t sc = (int64_t)blk * p.hkv + at % per_row / per_head;
-        const float sk = __ldg(p.scales[0] + sc), sv = __ldg(p.scales[1] + sc);
+    if (threadIdx.x == 0 && part == 0) {
+      p.tables[w] = (int32_t)w;
+      if (!have) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
+    }
+    const int loads = tokens * per_row;  // of K, and as many of V
+    const int share = p.share * kWidenLoads * kWidenThreads;
+    const int end = min(2 * loads, (part + 1) * share);
+    for (int i0 = part * share + threadIdx.x; i0 < end; i0 += kWidenLoads * kWidenThreads) {
+      uint4 raw[kWidenLoads];
+      float sk[kWidenLoads], sv[kWidenLoads];
+#pragma unroll
+      for (int k = 0; k < kWidenLoads; ++k) {
+        const int i = i0 + k * kWidenThreads;
+        raw[k] = make_uint4(0, 0, 0, 0);
+        sk[k] = sv[k] = 0.f;
+        if (have && i < end) {
+          const bool is_v = i >= loads;
+          const int at = is_v ? i - loads : i;
+          raw[k] = __ldg(reinterpret_cast<const uint4*>(p.codes[is_v]) + (int64_t)blk * p.block_size * per_row + at);
+          const int64_t sc = (int64_t)blk * p.hkv + at % per_row / per_head;
+          sk[k] = __ldg(p.scales[0] + sc);
+          sv[k] = __ldg(p.scales[1] + sc);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kWidenLoads; ++k) {
+        const int i = i0 + k * kWidenThreads;
+        if (i >= end) break;
+        const bool is_v = i >= loads;
+        const int at = is_v ? i - loads : i;
         // A NaN value block shows through the scores alone: rows that do not see it would
         // otherwise meet it as 0 * NaN in P V.
-        s = is_v ? (sv == sv ? sv : 0.f) : (sv == sv ? sk : sv);
-      }
-      uint32_t words[8];
-      const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+        const float s = is_v ? (sv[k] == sv[k] ? sv[k] : 0.f) : (sv[k] == sv[k] ? sk[k] : sv[k]);
+        uint32_t words[8];
+        const uint32_t in[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t two = fp8x2_to_f16x2((uint16_t)(in[k >> 1] >> (16 * (k & 1))));
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&two));
-        words[k] = pack2<T>(bounded<T>(x.x * s), bounded<T>(x.y * s));
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t two = fp8x2_to_f16x2((uint16_t)(in[e >> 1] >> (16 * (e & 1))));
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&two));
+          words[e] = pack2<T>(bounded<T>(x.x * s), bounded<T>(x.y * s));
+        }
+        uint4* to = reinterpret_cast<uint4*>(p.wide[is_v]) + (w * p.block_size * per_row + at) * 2;
+        to[0] = make_uint4(words[0], words[1], words[2], words[3]);
+        to[1] = make_uint4(words[4], words[5], words[6], words[7]);
       }
-      uint4* to = reinterpret_cast<uint4*>(p.wide[is_v]) + (w * p.block_size * per_row + at) * 2;
-      to[0] = make_uint4(words[0], words[1], words[2], words[3]);
-      to[1] = make_uint4(words[4], words[5], words[6], words[7]);
     }
   }
 }
@@ -362,6 +387,15 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     w.block_tables = block_tables;
     w.bt_stride = block_table_stride;
     w.width = (int)width;
+    const int64_t most = (int64_t)b2p_host::sm_count() * 8;
+    const int64_t blocks = (int64_t)num_seqs * width;
+    // rounds that a block takes; it is cut into pieces where the call's own rows do not fill the CTAs
+    const int rounds = (int)(((int64_t)2 * block_size * num_kv_heads * head_dim / 16 + kWidenLoads * kWidenThreads - 1) /
+                             (kWidenLoads * kWidenThreads));
+    const int64_t wanted = most * block_size / total_q + 1;
+    w.parts = (int)(wanted < rounds ? wanted : rounds);
+    w.share = (rounds + w.parts - 1) / w.parts;
+    w.parts = (rounds + w.share - 1) / w.share;
     w.cu = cu_seqlens_q;
     w.ctx = context_lens;
     w.out = static_cast<uint8_t*>(out);
@@ -381,9 +415,7 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
                                      align256((size_t)splits * total_q * num_q_heads * head_dim * 4));
     w.num_lse = splits > 1 ? (int64_t)splits * total_q * num_q_heads : 0;
     w.no_weight = b2p_prefill_no_weight();
-    const int64_t most = (int64_t)b2p_host::sm_count() * 8;
-    const int64_t blocks = (int64_t)num_seqs * width;
-    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    const unsigned grid = (unsigned)(blocks * w.parts < most ? blocks * w.parts : most);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == B2P_BF16)
       widen_histories<__nv_bfloat16><<<grid, kWidenThreads, 0, s>>>(w);

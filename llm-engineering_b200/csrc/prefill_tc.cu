@@ -459,6 +459,9 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
+  // Where this launch may start early (after the kernel that makes a 16-bit copy of an 8-bit
+  // history), nothing global has been read so far.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // An item as seen by the consumer warps: wait for its slot, copy it, hand the slot back.
   auto take_item = [&](int i, ItemInfo& it) -> bool {
@@ -1251,8 +1254,21 @@ int launch_prefill(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
   if (fit < 0) return B2P_EUNSUPPORTED;
   dim3 grid((unsigned)b2p_host::sm_count());
   void* args[] = {&qmap, &kmap, &vmap, &p};
-  e = cudaLaunchKernel(fn, grid, dim3(kThreads), args, (size_t)smem,
-                       static_cast<cudaStream_t>(stream));
+  if (claims == nullptr) {
+    e = cudaLaunchKernel(fn, grid, dim3(kThreads), args, (size_t)smem, static_cast<cudaStream_t>(stream));
+  } else {  // the set-up above runs while the kernel before it ends
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelExC(&cfg, fn, args);
+  }
   if (e != cudaSuccess) return b2p_host::record_error(e);
   const int lrc = b2p_host::check_launch();
   if (lrc != B2P_OK || splits == 1) return lrc;
