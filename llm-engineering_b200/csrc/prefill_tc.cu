@@ -245,9 +245,9 @@ struct SeqTiles {
 };
 
 __device__ __forceinline__ SeqTiles seq_tiles_global(const PrefillParams& p, int s) {
-  const int q0 = __ldg(p.cu_q + s);
-  const int q = __ldg(p.cu_q + s + 1) - q0;
-  const int ctx = __ldg(p.ctx + s);
+  const int q0 = __ldcg(p.cu_q + s);
+  const int q = __ldcg(p.cu_q + s + 1) - q0;
+  const int ctx = __ldcg(p.ctx + s);
   SeqTiles t;
   t.nt = q > 0 ? ceil_div(q, kM) : 0;
   t.c = ctx > q ? ceil_div(ctx - q, kN) : 0;
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
   // Where this launch may start early (after the kernel that makes a 16-bit copy of an 8-bit
-  // history), nothing global has been read so far.
+  // history), nothing global has been read so far, and lengths and tables come from L2.
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // An item as seen by the consumer warps: wait for its slot, copy it, hand the slot back.
@@ -537,9 +537,9 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
           it.kvh = r / pairs;
           it.qh_a = it.kvh * p.group + 2 * pr;
           it.qh_b = 2 * pr + 1 < p.group ? it.qh_a + 1 : -1;
-          it.q0 = __ldg(p.cu_q + seq);
-          it.qlen = __ldg(p.cu_q + seq + 1) - it.q0;
-          it.ctx = __ldg(p.ctx + seq);
+          it.q0 = __ldcg(p.cu_q + seq);
+          it.qlen = __ldcg(p.cu_q + seq + 1) - it.q0;
+          it.ctx = __ldcg(p.ctx + seq);
           it.rows_valid = min(kM, it.qlen - tile * kM);
           it.pos0 = it.ctx - it.qlen + tile * kM;  // position of the tile's first row
           const int last_pos = it.pos0 + it.rows_valid - 1;
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_tc(const __grid_consta
           const int at = kSplit ? sb + kt0 * kSubPerTile : sb;
           const int64_t col = at / spb;
           int32_t blk = -1;
-          if ((int64_t)sb * kSub < it.ctx && col < p.bt_stride) blk = __ldg(bt + col);
+          if ((int64_t)sb * kSub < it.ctx && col < p.bt_stride) blk = __ldcg(bt + col);
           if ((int64_t)sb * kSub < it.ctx && (blk < 0 || (int64_t)blk >= p.num_blocks)) {
             set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
             blk = -1;
