@@ -24,9 +24,13 @@
 //    values 2^-28 below a row's largest lose bits).
 //  * ks goes into the scores' fp32 factor. vs goes into P before P is rounded to f16 (11 bits),
 //    against a reference of its own: m_y tracks the largest score + log2(vs), as m_x does the
-//    scores, so the weights that matter keep their 11 bits whatever the spread of the scales.
-//    References only move when a score passes them by 2^8 (one warp vote per tile instead of
-//    shuffles and a rescale of O).
+//    scores. References only move when a score passes them by 2^4 (one warp vote per tile
+//    instead of shuffles and a rescale of O), and P vs is kept times 2^10, so that the largest
+//    lies in [2^10, 2^15) of f16's [2^-14, 2^16): weights down to 2^-24 of the largest keep their
+//    11 bits, smaller ones are rounded by 2^-35 of it. That matters where one key outweighs the
+//    others and its value is small (an attention sink): the output is then made of small
+//    weights, which l, a sum in fp32, counts in full. (With a slack of 2^8 and P as it is, weights
+//    of 2^-20.5 lost 4 % and those of 2^-25 were zero.)
 //  * Sequences cut by range boundaries leave partial records (O scaled into [-1, 1], then m_x, the
 //    sum and the scale in fp32) in shared memory. When a CTA's warps are through, they merge
 //    their records together, a 16-dim chunk per warp: sequences that lie inside the CTA's range
@@ -46,7 +50,8 @@ using namespace b2p;
 constexpr int kSub = 16;   // tokens per TMA box (any block size that is a multiple of 16)
 constexpr int kTile = 32;  // tokens per stage
 constexpr float kNoMax = -1e30f;     // log2 weight of a record that saw nothing
-constexpr float kSlack = 8.0f;       // log2 units a score may pass its reference by
+constexpr float kSlack = 4.0f;       // log2 units a score may pass its reference by
+constexpr float kLift = 10.0f;       // log2 of what P vs is multiplied by: 2^(kSlack + kLift + 1) fits f16
 constexpr int kL2Prefetch = 4;       // tiles per warp prefetched into L2 before the launch wait
 
 struct Fp8Params {
@@ -588,8 +593,9 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 
   int ncut = 0;  // records left (at most the unit's first and last segment)
 
-  // Rows of one virtual sequence from O^T fragments: out = O * factor.
-  auto write_out = [&](const Virtual& t, float (&o)[kChunks][NT][4], float (&f)[NT][2]) {
+  // Rows of one virtual sequence from O^T fragments: out = (O * f) * g. (Two factors: their product
+  // may lie below the normal range where the output does not.)
+  auto write_out = [&](const Virtual& t, float (&o)[kChunks][NT][4], float (&f)[NT][2], float (&g)[NT][2]) {
 #pragma unroll
     for (int nn = 0; nn < NT; ++nn) {
 #pragma unroll
@@ -602,7 +608,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
           *reinterpret_cast<uint32_t*>(orow + i * 16 + 2 * g8) =
-              pack2<T>(o[i][nn][cc] * f[nn][cc], o[i][nn][2 + cc] * f[nn][cc]);
+              pack2<T>(o[i][nn][cc] * f[nn][cc] * g[nn][cc], o[i][nn][2 + cc] * f[nn][cc] * g[nn][cc]);
       }
     }
   };
@@ -812,7 +818,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
             }
             mx[nn][cc] += dx;
             slack[nn][cc] += dy - dx;
-            gy[nn][cc] = fast_exp2(kSlack - slack[nn][cc]);  // 2^(m_x - m_y)
+            gy[nn][cc] = fast_exp2(kSlack + kLift - slack[nn][cc]);  // 2^(m_x - m_y + kLift)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               s[h][nn][cc] -= dx;
@@ -820,7 +826,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
             }
           }
       }
-      // ---- P = 2^(x - m_x); its f16 copy carries vs against m_y
+      // ---- P = 2^(x - m_x); its f16 copy carries vs and 2^kLift against m_y
       uint32_t pb[2][NT][2];
 #pragma unroll
       for (int nn = 0; nn < NT; ++nn) {
@@ -881,13 +887,15 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
         l[nn][1] += __shfl_xor_sync(0xffffffffu, l[nn][1], o);
       }
     if (lb0 == 0 && lb1 == ntl) {
-      float f[NT][2];
+      float f[NT][2], g[NT][2];
 #pragma unroll
       for (int nn = 0; nn < NT; ++nn)
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc)
-          f[nn][cc] = l[nn][cc] > 0.f ? fast_exp2(slack[nn][cc] - kSlack) / l[nn][cc] : 0.f;
-      write_out(t, acc, f);
+        for (int cc = 0; cc < 2; ++cc) {
+          f[nn][cc] = l[nn][cc] > 0.f ? 1.f / l[nn][cc] : 0.f;
+          g[nn][cc] = fast_exp2(slack[nn][cc] - (kSlack + kLift));  // 2^(m_y - m_x - kLift)
+        }
+      write_out(t, acc, f, g);
     } else {
       const bool in_ring = seg_end == r.end;
       float* rec = record_of(warp, in_ring);
@@ -912,7 +920,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
             Rec::put_stats(rec, nn * 8 + 2 * t4 + cc, weight_of(mx[nn][cc], l[nn][cc]),
-                           l[nn][cc] > 0.f ? top[cc] * (fast_exp2(slack[nn][cc] - kSlack) / l[nn][cc]) : 0.f);
+                           l[nn][cc] > 0.f ? top[cc] / l[nn][cc] * fast_exp2(slack[nn][cc] - (kSlack + kLift)) : 0.f);
           }
         }
       }
