@@ -713,7 +713,8 @@ def verify_drafts(
     when every draft is certain (prompt lookup, greedy drafts). Draft j stands while
     ``accept_draws[j] * q_j(x_j) < p_j(x_j)``; one more token is drawn with ``sample_draws[i]``
     from max(p - q, 0) of the first rejected row, or from p of the last row. Draws are fp32 in
-    [0, 1). Returns (tokens, accepted): int64 (num_seqs, max_drafts + 1), the standing drafts, then
+    [0, 1). NaN and negative probabilities, in either tensor, count as zero. Returns (tokens,
+    accepted): int64 (num_seqs, max_drafts + 1), the standing drafts, then
     the drawn token, then -1; and int32 (num_seqs,), how many drafts stand.
     """
     index = _index_of("target_probs", target_probs)

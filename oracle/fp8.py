@@ -110,7 +110,10 @@ def attend(q, kc, ks, vc, vs, block_size, tables, q_lens, ctx, scale):
 
 
 def verify(target, draft, tokens, cu, accept, sample, max_drafts):
-    """(tokens, accepted) as lists; target/draft float64 arrays, draft None for certain drafts."""
+    """(tokens, accepted) as lists; target/draft float64 arrays, draft None for certain drafts.
+    NaN and negative entries of either count as zero."""
+    target = np.where(target > 0, target, 0.0)
+    draft = None if draft is None else np.where(draft > 0, draft, 0.0)
     out, counts = [], []
     for i in range(len(cu) - 1):
         k, n = cu[i + 1] - cu[i], 0
@@ -125,7 +128,6 @@ def verify(target, draft, tokens, cu, accept, sample, max_drafts):
                 break
             n += 1
         p = target[cu[i] + i + n]
-        p = np.where(p > 0, p, 0.0)
         r = p
         if n < k:
             t = cu[i] + n
