@@ -318,7 +318,8 @@ B2P_API int b2p_kv_write_fp8(const void* keys, int64_t k_tok_stride, int64_t k_h
 
 /*
  * Rows of the given slots as values of `dtype`: keys, values [num_rows, num_kv_heads, head_dim],
- * contiguous. A negative slot gives zeros; one past the pool too, and sets B2P_DEV_SLOT_RANGE.
+ * contiguous. A negative slot gives zeros; one past the pool too, and sets B2P_DEV_SLOT_RANGE. A
+ * value past f16's range reads as f16's largest finite one (f16 rows from 63,488 up are held as 65,536).
  */
 B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, const float* key_scales,
                  const float* value_scales, const int32_t* slot_mapping, int64_t num_rows,

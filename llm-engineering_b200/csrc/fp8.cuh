@@ -10,6 +10,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b2p {
@@ -50,6 +52,20 @@ __device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint16_t two) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
+}
+
+// Two values of the cache (codes times scales) as a pair of T. f16 rows from 63,488 up are stored as
+// 65,536 (half a step of their code up), which is past f16's largest finite value: 65,504 stands
+// for it, and for everything above it in a pool that other types' rows went into. NaN stays NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_values(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  } else {
+    return pack2<T>(lo, hi);
+  }
 }
 
 }  // namespace b2p

@@ -489,8 +489,8 @@ __global__ void __launch_bounds__(256) kv_read_fp8_rows(const ReadFp8Params p) {
           reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
           reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
         } else {
-          *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
-                                                      pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+          *reinterpret_cast<uint4*>(out) = make_uint4(pack_values<T>(x[0], x[1]), pack_values<T>(x[2], x[3]),
+                                                      pack_values<T>(x[4], x[5]), pack_values<T>(x[6], x[7]));
         }
       }
     }

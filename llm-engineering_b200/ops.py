@@ -533,7 +533,8 @@ def kv_read_fp8(
     err_flag: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows of the given slots (int32) as values of ``dtype``: (keys, values), each
-    (rows, kv_heads, head_dim). Negative slots give zero rows."""
+    (rows, kv_heads, head_dim). Negative slots give zero rows; values past f16's range read as its
+    largest finite one."""
     index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
                                                      value_scales, block_size)
     _vector(index, "slot_mapping", slot_mapping, torch.int32)
