@@ -329,8 +329,8 @@ B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, cons
 
 /*
  * Attention over the 8-bit cache. Arguments as in b2p_paged_decode and b2p_paged_prefill; dtype is
- * that of q and out, scale must not be negative. Rows without a key to see (context 0) are zeros
- * and set B2P_DEV_LENGTH; offsets outside q's rows set it too, a context longer than its table row
+ * that of q and out, scale must not be negative. f16 outputs past its range are its largest finite
+ * value. Rows without a key to see (context 0) are zeros and set B2P_DEV_LENGTH; offsets outside q's rows set it too, a context longer than its table row
  * sets B2P_DEV_BLOCK_RANGE.
  *   workspace : b2p_paged_fp8_workspace_size() bytes, 16-byte aligned, zero before its first use
  *               and zeroed again after B2P_DEV_WAIT_TIMEOUT; every completed call leaves it ready

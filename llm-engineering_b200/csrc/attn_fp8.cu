@@ -87,6 +87,13 @@ struct WidenParams {
   int32_t* err;
 };
 
+// f16 keeps 65,472 where a product passes it (the next stored value is 65,536): 2^-11 below f16's largest
+// finite value, which is what the rounding of the weights in P V may add to a mean.
+template <typename T>
+__device__ __forceinline__ float bounded(float x) {
+  return std::is_same<T, __half>::value ? (x > 65472.f ? 65472.f : x < -65472.f ? -65472.f : x) : x;
+}
+
 __device__ __forceinline__ int row_within(const WidenParams& p, int row) {
   return (int)min(max((int64_t)row, (int64_t)0), p.num_rows);
 }
@@ -203,7 +210,7 @@ __global__ void __launch_bounds__(kWidenThreads, 8) widen_histories(const WidenP
         for (int e = 0; e < 8; ++e) {
           const uint32_t two = fp8x2_to_f16x2((uint16_t)(in[e >> 1] >> (16 * (e & 1))));
           const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&two));
-          words[e] = pack_values<T>(x.x * s, x.y * s);
+          words[e] = pack2<T>(bounded<T>(x.x * s), bounded<T>(x.y * s));
         }
         uint4* to = reinterpret_cast<uint4*>(p.wide[is_v]) + (w * p.block_size * per_row + at) * 2;
         to[0] = make_uint4(words[0], words[1], words[2], words[3]);

@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_fp8_simt(const SimtFp8
 #pragma unroll
   for (int k = 0; k < kMaxD / 32; ++k) {
     const int d = lane + 32 * k;
-    if (d < D) orow[d] = from_f32<T>(acc[k] * inv);
+    if (d < D) orow[d] = value_as<T>(acc[k] * inv);
   }
 }
 

@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
           *reinterpret_cast<uint32_t*>(orow + i * 16 + 2 * g8) =
-              pack2<T>(o[i][nn][cc] * f[nn][cc] * g[nn][cc], o[i][nn][2 + cc] * f[nn][cc] * g[nn][cc]);
+              pack_values<T>(o[i][nn][cc] * f[nn][cc] * g[nn][cc], o[i][nn][2 + cc] * f[nn][cc] * g[nn][cc]);
       }
     }
   };
@@ -971,7 +971,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_rows_fp8(const __grid_constan
       const float f = l[cc] > 0.f ? 1.f / l[cc] : 0.f;
       T* orow = reinterpret_cast<T*>(p.out) + (int64_t)(row0 + row) * p.o_tok +
                 (int64_t)(head * p.group + col0 + c - row * p.group) * p.o_head;
-      *reinterpret_cast<uint32_t*>(orow + i * 16 + 2 * g8) = pack2<T>(o[cc] * f, o[2 + cc] * f);
+      *reinterpret_cast<uint32_t*>(orow + i * 16 + 2 * g8) = pack_values<T>(o[cc] * f, o[2 + cc] * f);
     }
   };
   // The warp's share of the pieces of the groups in `heads`.

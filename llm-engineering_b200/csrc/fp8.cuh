@@ -54,7 +54,7 @@ __device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint16_t two) {
   return r;
 }
 
-// Two values of the cache (codes times scales) as a pair of T. f16 rows from 63,488 up are stored as
+// Two values of the cache (codes times scales, or means of them) as a pair of T. f16 rows from 63,488 up are stored as
 // 65,536 (half a step of their code up), which is past f16's largest finite value: 65,504 stands
 // for it, and for everything above it in a pool that other types' rows went into. NaN stays NaN.
 template <typename T>
@@ -66,6 +66,12 @@ __device__ __forceinline__ uint32_t pack_values(float lo, float hi) {
   } else {
     return pack2<T>(lo, hi);
   }
+}
+
+template <typename T>
+__device__ __forceinline__ T value_as(float x) {  // the same for one value
+  return std::is_same<T, __half>::value ? from_f32<T>(x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x)
+                                        : from_f32<T>(x);
 }
 
 }  // namespace b2p
