@@ -330,18 +330,25 @@ B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, cons
 /*
  * Attention over the 8-bit cache. Arguments as in b2p_paged_decode and b2p_paged_prefill; dtype is
  * that of q and out, scale must not be negative. f16 outputs past its range are its largest finite
- * value. Rows without a key to see (context 0) are zeros and set B2P_DEV_LENGTH; offsets outside q's rows set it too, a context longer than its table row
- * sets B2P_DEV_BLOCK_RANGE.
+ * value. Rows without a key to see (context 0) are zeros and set B2P_DEV_LENGTH; offsets outside
+ * q's rows set it too, a context longer than its table row sets B2P_DEV_BLOCK_RANGE.
  *   workspace : b2p_paged_fp8_workspace_size() bytes, 16-byte aligned, zero before its first use
  *               and zeroed again after B2P_DEV_WAIT_TIMEOUT; every completed call leaves it ready
  *               for the next one on the stream, whatever its shape. Calls that may overlap (two
  *               streams, two captured graphs) need one each.
  *   max_q_len : upper bound of the q_len_i; a longer sequence sets B2P_DEV_LENGTH and its rows
  *               are left alone, or are computed all the same.
- *   scratch   : b2p_paged_prefill_fp8_scratch_size() bytes (0 where the call needs none), any
+ *   scratch   : b2p_paged_prefill_fp8_pool_scratch_size() bytes (0 where the call needs none), any
  *               contents: many rows run on a 16-bit copy of the histories, made by the call.
- *               table_width is block_table_stride.
+ *               table_width is block_table_stride, num_slots the pool's: the copy has a block for
+ *               each table entry or for each of the pool's blocks, whichever are fewer.
+ *               b2p_paged_prefill_fp8_scratch_size() is enough for a pool of any size. Calls of few
+ *               query tiles cut the keys into runs by the table's width: tables no wider than
+ *               their longest history serve them best.
  */
+B2P_API size_t b2p_paged_prefill_fp8_pool_scratch_size(int num_seqs, int64_t total_q,
+                 int64_t table_width, int64_t num_slots, int num_q_heads, int num_kv_heads,
+                 int head_dim, int block_size, int max_q_len, int dtype);
 B2P_API size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total_q,
                  int64_t table_width, int num_q_heads, int num_kv_heads, int head_dim, int block_size, int max_q_len,
                  int dtype);

@@ -51,6 +51,7 @@ EXPORTED_SYMBOLS = (
     "b2p_paged_fp8_workspace_size",
     "b2p_paged_decode_fp8",
     "b2p_paged_prefill_fp8_scratch_size",
+    "b2p_paged_prefill_fp8_pool_scratch_size",
     "b2p_paged_prefill_fp8",
     "b2p_verify_drafts",
     "b2p_verify_drafts_greedy",
@@ -127,6 +128,9 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "b2p_paged_prefill_fp8_scratch_size": (
         _sz, [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32],
+    ),
+    "b2p_paged_prefill_fp8_pool_scratch_size": (
+        _sz, [_i32, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32],
     ),
     "b2p_paged_prefill_fp8": (
         _i32,

@@ -66,8 +66,8 @@ constexpr int kWidenLoads = 2;  // loads that a thread has in flight
 struct WidenParams {
   const uint8_t* codes[2];  // layer bases of K and V
   const float* scales[2];
-  uint8_t* wide[2];         // scratch pools [num_seqs * width blocks]
-  int32_t* tables;          // scratch block tables [num_seqs, width]
+  uint8_t* wide[2];         // scratch pools
+  int32_t* tables;          // scratch block tables [num_seqs, width]; null: blocks keep their ids
   const int32_t* block_tables;
   int64_t bt_stride;
   int width;
@@ -100,10 +100,12 @@ __device__ __forceinline__ int row_within(const WidenParams& p, int row) {
 
 // A CTA takes pieces of the used blocks of all histories in turn (found by a scan of the lengths,
 // 32 sequences at a time: with one CTA per table entry, most of a ragged batch's are empty, 35 us
-// against 22 on 32 prompts) and writes their codes as 16-bit rows into the scratch block that the
-// // scratch table gives them. A piece is a whole block where there are many, else down to what the
-// CTA's threads have in flight at once (one sequence of 210 rows and 4 heads in blocks of 64: the call
-// takes 17.9 us, 22.5 with whole blocks). Memory-bound: 1 byte read and 2 written per element.
+// against 22 on 32 prompts) and writes their codes as 16-bit rows: into a scratch block of the entry's
+// own, which the scratch table names, or into a scratch pool with the blocks' own ids, whichever pool
+// is smaller. (With their own ids, sequences that share a block write the same bytes to it.) A piece is
+// a whole block where there are many, else down to what the CTA's threads have in flight at once
+// (one sequence of 210 rows and 4 heads in blocks of 64: the call takes 17.9 us, 22.5 with whole
+// blocks). Memory-bound: 1 byte read and 2 written per element.
 template <typename T>
 __global__ void __launch_bounds__(kWidenThreads, 8) widen_histories(const WidenParams p) {
   __shared__ int found[2];  // sequence (-1: no block left) and block number
@@ -167,14 +169,16 @@ __global__ void __launch_bounds__(kWidenThreads, 8) widen_histories(const WidenP
     __syncthreads();
     const int seq = found[0], col = found[1], part = (int)(unit % p.parts);
     if (seq < 0) return;
-    const int64_t w = (int64_t)seq * p.width + col;
+    const int64_t entry = (int64_t)seq * p.width + col;
     const int tokens = min(p.block_size, __ldg(p.ctx + seq) - col * p.block_size);
     const int32_t blk = __ldg(p.block_tables + (int64_t)seq * p.bt_stride + col);
     const bool have = blk >= 0 && blk < p.num_blocks;
     if (threadIdx.x == 0 && part == 0) {
-      p.tables[w] = (int32_t)w;
+      if (p.tables != nullptr) p.tables[entry] = (int32_t)entry;
       if (!have) set_device_error(p.err, B2P_DEV_BLOCK_RANGE);
     }
+    if (p.tables == nullptr && !have) continue;  // the tile kernel finds the bad id itself
+    const int64_t w = p.tables != nullptr ? entry : blk;
     const int loads = tokens * per_row;  // of K, and as many of V
     const int share = p.share * kWidenLoads * kWidenThreads;
     const int end = min(2 * loads, (part + 1) * share);
@@ -223,16 +227,33 @@ __global__ void __launch_bounds__(kWidenThreads, 8) widen_histories(const WidenP
 constexpr int kMostSplits = 8;
 constexpr int kRunTiles = 8;
 
-// Scratch of the widened form: the block tables with the checked offsets and lengths and the claim
-// counters, then K, then V, then (split calls) the runs' results and weights.
+// Scratch of the widened form: the checked offsets and lengths, the claim counters and (blocks by table
+// entry) the block tables, then K, then V, then (split calls) the runs' results and weights. The
+// 16-bit copies take as many blocks as the tables have entries or as the pool has blocks, whichever is
+// less: tables are as wide as their longest sequence, and a batch of unlike lengths would
+// otherwise ask for many times what it holds (32 prompts of which one has 131,072 tokens, 8 heads of
+// 128: 17 GB).
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
-size_t table_bytes(int num_seqs, int64_t width) {
-  return align256(((size_t)num_seqs * width + 2 * (size_t)num_seqs + 1 + 2) * 4);
-}
+struct Scratch {
+  int64_t blocks;  // of the 16-bit copies
+  bool own_ids;    // they are the pool's own
+  size_t tables, pool, part, lse;  // bytes
+  size_t total() const { return tables + 2 * pool + part + lse; }
+};
 
-size_t wide_bytes(int num_seqs, int64_t width, int num_kv_heads, int head_dim, int block_size) {
-  return align256((size_t)num_seqs * width * block_size * num_kv_heads * head_dim * 2);
+Scratch scratch_of(int num_seqs, int64_t width, int64_t pool_blocks, int num_kv_heads, int head_dim, int block_size,
+                   int splits, int64_t total_q, int num_q_heads) {
+  Scratch c;
+  const int64_t entries = (int64_t)num_seqs * width;
+  c.own_ids = pool_blocks < entries;
+  c.blocks = c.own_ids ? pool_blocks : entries;
+  c.tables = align256(((c.own_ids ? 0 : (size_t)entries) + 2 * (size_t)num_seqs + 1 + 2) * 4);
+  c.pool = align256((size_t)c.blocks * block_size * num_kv_heads * head_dim * 2);
+  const size_t rows = splits > 1 ? (size_t)splits * total_q * num_q_heads : 0;
+  c.part = align256(rows * head_dim * 4);
+  c.lse = align256(rows * 4);
+  return c;
 }
 
 // Runs that every (query tile, pair of heads) item's keys are cut into, where a call has too few
@@ -319,19 +340,26 @@ extern "C" int b2p_paged_decode_fp8(const void* q, int64_t q_tok_stride, int64_t
                            dtype, err_flag, stream);
 }
 
-extern "C" size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total_q, int64_t table_width, int num_q_heads,
-                                                     int num_kv_heads, int head_dim, int block_size,
-                                                     int max_q_len, int dtype) {
-  if (num_seqs <= 0 || total_q <= 0 || table_width <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
-      block_size <= 0 || max_q_len < 0 || num_q_heads % num_kv_heads != 0 || !tile_shape(head_dim, block_size, dtype))
+extern "C" size_t b2p_paged_prefill_fp8_pool_scratch_size(int num_seqs, int64_t total_q, int64_t table_width,
+                                                          int64_t num_slots, int num_q_heads, int num_kv_heads,
+                                                          int head_dim, int block_size, int max_q_len, int dtype) {
+  if (num_seqs <= 0 || total_q <= 0 || table_width <= 0 || num_slots <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      head_dim <= 0 || block_size <= 0 || max_q_len < 0 || num_q_heads % num_kv_heads != 0 ||
+      !tile_shape(head_dim, block_size, dtype))
     return 0;
   if (b2p_rows_fp8_takes(num_q_heads / num_kv_heads, head_dim, block_size, dtype, max_q_len)) return 0;
   const int splits = key_splits(num_seqs, total_q, table_width, num_q_heads, num_kv_heads, block_size);
-  const size_t parts = splits > 1 ? align256((size_t)splits * total_q * num_q_heads * head_dim * 4) +
-                                        align256((size_t)splits * total_q * num_q_heads * 4)
-                                  : 0;
-  return table_bytes(num_seqs, table_width) +
-         2 * wide_bytes(num_seqs, table_width, num_kv_heads, head_dim, block_size) + parts;
+  return scratch_of(num_seqs, table_width, num_slots / block_size, num_kv_heads, head_dim, block_size, splits, total_q,
+                    num_q_heads)
+      .total();
+}
+
+// The same for any pool: one with more blocks than the tables have entries asks for the most.
+extern "C" size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total_q, int64_t table_width, int num_q_heads,
+                                                     int num_kv_heads, int head_dim, int block_size,
+                                                     int max_q_len, int dtype) {
+  return b2p_paged_prefill_fp8_pool_scratch_size(num_seqs, total_q, table_width, INT64_MAX, num_q_heads, num_kv_heads,
+                                                 head_dim, block_size, max_q_len, dtype);
 }
 
 extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -362,13 +390,12 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
                         out_tok_stride, out_head_stride, workspace, workspace_size, dtype,
                         err_flag, stream);
   const int64_t width = block_table_stride;
-  if (tile_shape(head_dim, block_size, dtype) && aligned(key_cache, 16) && aligned(value_cache, 16) &&
-      (int64_t)num_seqs * width * block_size <= 0x7fffffffLL && width > 0 &&
+  if (tile_shape(head_dim, block_size, dtype) && aligned(key_cache, 16) && aligned(value_cache, 16) && width > 0 &&
       tile_rows_fit(q, q_tok_stride, q_head_stride, out, out_tok_stride, out_head_stride)) {
-    if (!scratch || scratch_size < b2p_paged_prefill_fp8_scratch_size(num_seqs, total_q, width, num_q_heads, num_kv_heads,
-                                                                      head_dim, block_size, max_q_len, dtype) ||
-        !aligned(scratch, 16))
-      return B2P_EWORKSPACE;
+    const int splits = key_splits(num_seqs, total_q, width, num_q_heads, num_kv_heads, block_size);
+    const Scratch need = scratch_of(num_seqs, width, num_slots / block_size, num_kv_heads, head_dim, block_size, splits,
+                                    total_q, num_q_heads);
+    if (!scratch || scratch_size < need.total() || !aligned(scratch, 16)) return B2P_EWORKSPACE;
     WidenParams w;
     const int64_t layer_codes = num_slots * num_kv_heads * head_dim;
     const int64_t layer_scales = num_slots / block_size * num_kv_heads;
@@ -377,14 +404,12 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     w.scales[0] = key_scales + layer_index * layer_scales;
     w.scales[1] = value_scales + layer_index * layer_scales;
     uint8_t* base = static_cast<uint8_t*>(scratch);
-    const size_t tables = table_bytes(num_seqs, width);
-    const size_t pool = wide_bytes(num_seqs, width, num_kv_heads, head_dim, block_size);
-    w.tables = reinterpret_cast<int32_t*>(base);
-    w.safe_cu = w.tables + num_seqs * width;
+    w.safe_cu = reinterpret_cast<int32_t*>(base);
     w.safe_ctx = w.safe_cu + num_seqs + 1;
     w.claims = w.safe_ctx + num_seqs;
-    w.wide[0] = base + tables;
-    w.wide[1] = base + tables + pool;
+    w.tables = need.own_ids ? nullptr : w.claims + 2;
+    w.wide[0] = base + need.tables;
+    w.wide[1] = base + need.tables + need.pool;
     w.block_tables = block_tables;
     w.bt_stride = block_table_stride;
     w.width = (int)width;
@@ -410,10 +435,8 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     w.block_size = block_size;
     w.num_blocks = num_slots / block_size;
     w.err = err_flag;
-    const int splits = key_splits(num_seqs, total_q, width, num_q_heads, num_kv_heads, block_size);
-    float* part = reinterpret_cast<float*>(base + tables + 2 * pool);
-    w.lse = reinterpret_cast<float*>(base + tables + 2 * pool +
-                                     align256((size_t)splits * total_q * num_q_heads * head_dim * 4));
+    float* part = reinterpret_cast<float*>(base + need.tables + 2 * need.pool);
+    w.lse = reinterpret_cast<float*>(base + need.tables + 2 * need.pool + need.part);
     w.num_lse = splits > 1 ? (int64_t)splits * total_q * num_q_heads : 0;
     w.no_weight = b2p_prefill_no_weight();
     const unsigned grid = (unsigned)(blocks * w.parts < most ? blocks * w.parts : most);
@@ -425,7 +448,8 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     const int wrc = b2p_host::check_launch();
     if (wrc != B2P_OK) return wrc;
     return b2p_prefill_tc_runs(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1],
-                               blocks * block_size, w.tables, width, w.safe_cu, w.safe_ctx, num_seqs,
+                               need.blocks * block_size, need.own_ids ? block_tables : w.tables, width,
+                               w.safe_cu, w.safe_ctx, num_seqs,
                                total_q, num_q_heads, num_kv_heads, head_dim, block_size, scale, out,
                                out_tok_stride, out_head_stride, dtype, err_flag, stream, w.claims,
                                splits, part, w.lse);

@@ -654,9 +654,11 @@ def paged_prefill_fp8(
     q: (rows, num_q_heads, head_dim); sequence i owns rows [cu_seqlens_q[i], cu_seqlens_q[i+1]) and
     row j of it sits at position ``context_lens[i] - q_len + j``. ``max_q_len`` bounds the q_len
     (rows of a longer sequence are flagged, or computed all the same). Rows of q that no sequence
-    owns are left alone in out. Calls of many rows widen the histories into a 16-bit copy of
-    ``num_seqs * block_tables.shape[1]`` blocks of one layer, allocated for the call (with fp32
-    partial results where few query tiles are spread over the SMs by their keys).
+    owns are left alone in out. Calls of many rows widen the histories into a 16-bit copy, allocated
+    for the call, of one layer's blocks: ``num_seqs * block_tables.shape[1]`` of them or as many as the
+    pool has, whichever are fewer (with fp32 partial results where few query tiles are spread over
+    the SMs by their keys, in runs sized by the tables' width: pass tables no wider than the
+    longest history).
     """
     index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
                                                      value_scales, block_size)
@@ -668,8 +670,8 @@ def paged_prefill_fp8(
     workspace = _fp8_workspace(index, workspace, n, hq, hkv, d, max_q_len)
     scratch, size = None, 0
     if max_q_len * hq > _row_columns() * hkv:
-        size = _lib.load().b2p_paged_prefill_fp8_scratch_size(n, total_q, width, hq, hkv, d,
-                                                              block_size, max_q_len, code)
+        size = _lib.load().b2p_paged_prefill_fp8_pool_scratch_size(
+            n, total_q, width, slots, hq, hkv, d, block_size, max_q_len, code)
         scratch = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     _call("b2p_paged_prefill_fp8", index, q.data_ptr(), qt, qh, key_cache.data_ptr(),
           value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
