@@ -84,6 +84,9 @@ class StepBatch:
     # the cache hook, since a block's scale depends on every row in it.
     key_scales: torch.Tensor | None = None
     value_scales: torch.Tensor | None = None
+    # The prefill executions' block tables for an 8-bit pool, as wide as those need: the call sizes
+    # its scratch and its runs of keys by the width, and decode rows' histories may be far longer.
+    prefill_tables: torch.Tensor | None = None
 
 
 def _phase_of(execution) -> str:
@@ -123,7 +126,7 @@ def paged_attention(module: torch.nn.Module, query: torch.Tensor, key: torch.Ten
                                batch.block_size, scaling, out=out[:nd],
                                workspace=batch.workspace, err_flag=batch.err)
         if nd < batch.num_execs:
-            k.paged_prefill_fp8(q, *pool, batch.block_tables[nd:], batch.cu_seqlens_q[nd:],
+            k.paged_prefill_fp8(q, *pool, batch.prefill_tables, batch.cu_seqlens_q[nd:],
                                 batch.context_lens[nd:], batch.max_q_len, batch.block_size,
                                 scaling, out=out, workspace=batch.workspace, err_flag=batch.err)
         return out.unsqueeze(0), None
@@ -408,9 +411,13 @@ class B200PagedModelRunner:
             tables = dev_i32[3 * n:].view(n, width)
             md = kernels.build_metadata(qlens, ctx, rows, tables, bs, total_q, 0, self._err)
         key_scales = getattr(self._storage, "key_scales", None)
+        prefill_tables = None
         if key_scales is not None:
             if d["block_size"] != self._storage.block_size:
                 raise ValueError("an 8-bit cache needs block-structured slot_ids")
+            if num_decode < n:
+                reach = max(-(-length // bs) for length in d["lengths"][num_decode:])
+                prefill_tables = tables[num_decode:, :reach].contiguous()
             need = kernels.fp8_workspace_size(n, self._hq, self._hkv, self._head_dim)
         else:
             need = kernels.decode_workspace_size(max(num_decode, 1), self._hq, self._hkv,
@@ -426,7 +433,8 @@ class B200PagedModelRunner:
             logit_indices=md["logit_indices"], workspace=self._workspace, err=self._err,
             fused_decode=(key_scales is None and num_decode > 0
                           and hasattr(kernels, "paged_decode_append")),
-            key_scales=key_scales, value_scales=getattr(self._storage, "value_scales", None))
+            key_scales=key_scales, value_scales=getattr(self._storage, "value_scales", None),
+            prefill_tables=prefill_tables)
         return batch, input_ids
 
     # ------------------------------------------------------------------ ModelRunner
