@@ -447,12 +447,12 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
       widen_histories<__half><<<grid, kWidenThreads, 0, s>>>(w);
     const int wrc = b2p_host::check_launch();
     if (wrc != B2P_OK) return wrc;
-    return b2p_prefill_tc_runs(q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1],
-                               need.blocks * block_size, need.own_ids ? block_tables : w.tables, width,
-                               w.safe_cu, w.safe_ctx, num_seqs,
-                               total_q, num_q_heads, num_kv_heads, head_dim, block_size, scale, out,
-                               out_tok_stride, out_head_stride, dtype, err_flag, stream, w.claims,
-                               splits, part, w.lse);
+    const int trc = b2p_prefill_tc_runs(
+        q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1], need.blocks * block_size,
+        need.own_ids ? block_tables : w.tables, width, w.safe_cu, w.safe_ctx, num_seqs, total_q, num_q_heads,
+        num_kv_heads, head_dim, block_size, scale, out, out_tok_stride, out_head_stride, dtype, err_flag, stream,
+        w.claims, splits, part, w.lse);
+    if (trc != B2P_EUNSUPPORTED) return trc;  // a device that the tile kernel does not fit: as b2p_paged_prefill does
   }
   if (dtype != B2P_F32) b2p_host::note_fallback(3);
   return b2p_attn_fp8_simt(q, q_tok_stride, q_head_stride, key_cache, value_cache, key_scales,
