@@ -61,7 +61,8 @@ enum b2p_device_error {
   B2P_DEV_BLOCK_RANGE = 2,  /* block id outside [0, num_slots/block_size) */
   B2P_DEV_WAIT_TIMEOUT = 4, /* a bounded mbarrier / flag wait gave up     */
   B2P_DEV_LENGTH = 8,       /* a context/query length that does not fit  */
-  B2P_DEV_TOKEN_RANGE = 16  /* drafted token id outside the vocabulary   */
+  B2P_DEV_TOKEN_RANGE = 16, /* drafted token id outside the vocabulary   */
+  B2P_DEV_VALUE_RANGE = 32  /* a stored value past the range of a 16-bit copy */
 };
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -339,7 +340,11 @@ B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, cons
  *   max_q_len : upper bound of the q_len_i; a longer sequence sets B2P_DEV_LENGTH and its rows
  *               are left alone, or are computed all the same.
  *   scratch   : b2p_paged_prefill_fp8_pool_scratch_size() bytes (0 where the call needs none), any
- *               contents: many rows run on a 16-bit copy of the histories, made by the call.
+ *               contents: many rows run on a copy of the histories in q's type, made by the call.
+ *               In f16 that holds what f16 rows leave in a pool. In a pool of other types' rows,
+ *               values past 65,536 set B2P_DEV_VALUE_RANGE and count as 65,472, and what lies below
+ *               2^-24 is lost; weights are f16 there as in b2p_paged_prefill, so those below 2^-25 of
+ *               a row's largest count as zero. (Few rows take codes and scales as they are.)
  *               table_width is block_table_stride, num_slots the pool's: the copy has a block for
  *               each table entry or for each of the pool's blocks, whichever are fewer.
  *               b2p_paged_prefill_fp8_scratch_size() is enough for a pool of any size. Calls of few

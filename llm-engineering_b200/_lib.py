@@ -29,6 +29,7 @@ DEV_BLOCK_RANGE = 2
 DEV_WAIT_TIMEOUT = 4
 DEV_LENGTH = 8
 DEV_TOKEN_RANGE = 16
+DEV_VALUE_RANGE = 32
 
 EXPORTED_SYMBOLS = (
     "b2p_version",

@@ -87,6 +87,8 @@ struct WidenParams {
   int32_t* err;
 };
 
+constexpr float kF16Scale = 146.f;  // 448 times a larger one may pass 65,536, the largest value of f16 rows
+
 // f16 keeps 65,472 where a product passes it (the next stored value is 65,536): 2^-11 below f16's largest
 // finite value, which is what the rounding of the weights in P V may add to a mean.
 template <typename T>
@@ -210,6 +212,16 @@ __global__ void __launch_bounds__(kWidenThreads, 8) widen_histories(const WidenP
         const float s = is_v ? (sv[k] == sv[k] ? sv[k] : 0.f) : (sv[k] == sv[k] ? sk[k] : sv[k]);
         uint32_t words[8];
         const uint32_t in[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        if (std::is_same<T, __half>::value && fabsf(s) > kF16Scale) {  // not from f16 rows, as a rule
+          bool past = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t two = fp8x2_to_f16x2((uint16_t)(in[e >> 1] >> (16 * (e & 1))));
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&two));
+            past |= fabsf(x.x * s) > 65536.f || fabsf(x.y * s) > 65536.f;
+          }
+          if (past) set_device_error(p.err, B2P_DEV_VALUE_RANGE);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t two = fp8x2_to_f16x2((uint16_t)(in[e >> 1] >> (16 * (e & 1))));

@@ -658,7 +658,8 @@ def paged_prefill_fp8(
     for the call, of one layer's blocks: ``num_seqs * block_tables.shape[1]`` of them or as many as the
     pool has, whichever are fewer (with fp32 partial results where few query tiles are spread over
     the SMs by their keys, in runs sized by the tables' width: pass tables no wider than the
-    longest history).
+    longest history). The copy is in q's type: with f16 queries over a pool that bf16 or fp32 rows
+    went into, values past 65,536 are flagged (B2P_DEV_VALUE_RANGE) and cut.
     """
     index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
                                                      value_scales, block_size)

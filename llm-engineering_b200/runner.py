@@ -551,7 +551,8 @@ class B200PagedModelRunner:
 
 _ERROR_BITS = ((1, "slot id outside the pool"), (2, "block id outside the pool"),
                (4, "a bounded wait gave up"), (8, "a length that does not fit"),
-               (16, "a drafted token outside the vocabulary"))
+               (16, "a drafted token outside the vocabulary"),
+               (32, "a stored value past the range of a 16-bit copy"))
 
 
 def _error_names(bits: int) -> list[str]:
