@@ -301,6 +301,7 @@ class B200PagedModelRunner:
         self._workspace = torch.zeros(16, dtype=torch.uint8, device=self._device)
         self._err = torch.zeros(1, dtype=torch.int32, device=self._device)
         self._mirror: _TableMirror | None = None
+        self._compactions = getattr(self._storage, "compactions", 0)
         self._k6_hidden: torch.Tensor | None = None
         self._k6_workspace: torch.Tensor | None = None
 
@@ -377,8 +378,10 @@ class B200PagedModelRunner:
             # rows of the device mirror (new blocks uploaded by sync); K4 gathers this step's
             # padded [n, width] tables from them
             keys = [(ex.sequence.request.request_id, ex.sequence.admissions) for ex in executions]
-            if self._mirror is None:
-                self._mirror = _TableMirror(dev)
+            compactions = getattr(self._storage, "compactions", 0)
+            if self._mirror is None or compactions != self._compactions:
+                self._mirror = _TableMirror(dev)  # also after the pool's pages have moved
+                self._compactions = compactions
             mirror_rows = self._mirror.sync(keys, d["tables"])
             width = max(1, max(-(-length // bs) for length in d["lengths"]))
             host = np.empty((3 * n,), dtype=np.int32)
@@ -521,7 +524,8 @@ class B200PagedModelRunner:
 
     def forget_tables(self) -> None:
         """Drop the device copy of the block tables (it only learns of new blocks, not of moved
-        ones): call it after ``PagedKVStorage.compact``; the next step uploads whole tables."""
+        ones): call it after moving pages by ``ops.compact_blocks``; the next step uploads whole
+        tables. (``PagedKVStorage.compact`` needs no call: the runner sees that it has run.)"""
         self._mirror = None
 
     @staticmethod

@@ -26,6 +26,7 @@ from . import ops
 class PagedKVStorage:
     key_scales: torch.Tensor | None = None
     value_scales: torch.Tensor | None = None
+    compactions = 0  # how often pages of this pool have moved
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int,
                  head_dim: int, dtype: torch.dtype, device: torch.device) -> None:
@@ -79,8 +80,9 @@ class PagedKVStorage:
     def compact(self, block_table) -> int:
         """Move the blocks of every request in ``block_table`` (engine.BlockTable) to the front of
         the pool, in every layer, and rewrite the tables and the block pool. Returns the number
-        of blocks in use. A runner that has run on this pool must drop the tables it keeps
-        (``B200PagedModelRunner.forget_tables``)."""
+        of blocks in use. A runner on this pool uploads its tables anew in its next step. (It
+        frees no memory: the pool's size is fixed. It is for programs that hand the pool's unused
+        end to something else, or that want pages in few places.)"""
         lists = list(block_table.tables().values())
         if block_table.block_size != self.block_size or block_table.pool.num_blocks != self.num_blocks:
             raise ValueError("block_table must be over this pool's blocks.")
@@ -99,6 +101,7 @@ class PagedKVStorage:
             self.value_scales, err_flag=err)
         if int(err.item()):
             raise RuntimeError("block_table names blocks outside the pool.")
+        self.compactions += 1
         block_table.apply_moves(new_ids.tolist())
         return int(live.item())
 

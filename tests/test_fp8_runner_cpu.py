@@ -67,3 +67,31 @@ def test_prompts_get_tables_as_wide_as_they_need(monkeypatch, decode, prompts):
     for table, ctx, contiguous in notes.decode:
         assert contiguous and ctx == lengths[:nd]
         assert [row[:len(b)].tolist() for row, b in zip(table, blocks)] == blocks[:nd]
+
+
+@pytest.mark.parametrize("make", [lambda: Fp8PagedKVStorage(2, 64, BS, 2, 16, torch.device("cpu")),
+                                  lambda: plain_storage()])
+def test_tables_are_uploaded_anew_after_a_compaction(monkeypatch, make):
+    """The device copy of the tables learns of new blocks only: moved ones would be read where they were."""
+    notes = Notes()
+    monkeypatch.setattr(runner_mod, "_ops", notes)
+    seen = []
+    monkeypatch.setattr(Notes, "build_metadata", staticmethod(
+        lambda *a, **k: seen.append(CpuKernels.build_metadata(*a, **k)) or seen[-1]))
+    storage = make()
+    runner = B200PagedModelRunner(tiny_model(), torch.device("cpu"), storage)
+    step = Execution("r", 40, 40, [9, 5, 30])
+    runner.forward([step])
+    assert seen[-1]["block_tables"][0].tolist() == [9, 5, 30]
+    storage.compactions += 1  # what compact() does when it has moved the pages
+    step.block_ids = (0, 1, 2)
+    runner.forward([step])
+    assert seen[-1]["block_tables"][0].tolist() == [0, 1, 2]
+
+
+def plain_storage():
+    from llm_engineering_b200.storage import PagedKVStorage
+
+    s = PagedKVStorage(2, 64, BS, 2, 16, torch.float32, torch.device("cpu"))
+    s.key_cache.zero_(), s.value_cache.zero_()
+    return s
