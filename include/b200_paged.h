@@ -296,7 +296,7 @@ B2P_API int b2p_lm_head_argmax(const void* hidden, int64_t hidden_row_stride, co
  * An element stands for code * scale of its (layer, block, head). The write below keeps every
  * scale a power of two: 2^e with the smallest e >= -110 for which the block's largest magnitude
  * is at most 448 * 2^e. A NaN or an infinity among a block's rows makes its scale NaN until the
- * block is started anew. Readers take any scale.
+ * block is started anew. Readers take any finite scale that is not negative, and NaN.
  *
  * K7 -- b2p_kv_write_fp8: sequence i appends rows [cu_seqlens_q[i], cu_seqlens_q[i+1]) of
  * keys/values (bf16, f16 or fp32; strides in elements) at positions context_lens[i] - q_len_i ..

@@ -4,10 +4,10 @@
 //
 // Few rows stream the codes (decode_fp8.cu). Many rows are bound by the tensor cores and read
 // every key tile once per 128-row query tile and head pair; there the histories are widened once
-// per call into a 16-bit scratch pool (22 us of the 750 below) and the 16-bit tile kernel
+// per call into a 16-bit scratch pool (23 us of the 777 below) and the 16-bit tile kernel
 // (prefill_tc.cu) runs on that. Widening inside the tile kernel instead, by two more warps that
 // fill its shared-memory tiles from the codes, repeats the conversion for every query tile and
-// head pair: 2351 us against 750 on 32 prompts of 64 to 8192 tokens.
+// head pair: 2351 us against 777 on 32 prompts of 64 to 8192 tokens.
 #include <type_traits>
 
 #include "fp8.cuh"

@@ -8,9 +8,10 @@
 // sequence touches only the first can hold older rows; where the new rows need a larger
 // scale there, the older codes are rounded to it in the same pass.
 //   e_new = max(e_old if the write leaves the block's first slot alone, e(amax of the new rows))
-// The work is pure streaming: every new row is read once, its codes are written once. A warp holds
-// its rows in registers between the two (16 rows of 128 take 8 16-byte pieces a lane); where they
-// do not fit it reads them again, from L2.
+// Every new row is read once, its codes are written once. A warp holds its rows in registers
+// between the two (16 rows of 128 take 8 16-byte pieces a lane); where they do not fit it reads them
+// again, from L2, piece by piece: 53,400 rows of 2 x 128 in bf16 take 22.6 us with blocks of 16 tokens,
+// 36.9 with 32 and 39.5 with 64 (d 64: 14.4 with 32, 20.6 with 64); in fp32 29.2 with 16, 53.7 with 32.
 #include <type_traits>
 
 #include "fp8.cuh"
