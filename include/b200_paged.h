@@ -345,11 +345,14 @@ B2P_API int b2p_kv_read_fp8(const void* key_cache, const void* value_cache, cons
  *               values past 65,536 set B2P_DEV_VALUE_RANGE and count as 65,472, and what lies below
  *               2^-24 is lost; weights are f16 there as in b2p_paged_prefill, so those below 2^-25 of
  *               a row's largest count as zero. (Few rows take codes and scales as they are.)
- *               table_width is block_table_stride, num_slots the pool's: the copy has a block for
- *               each table entry or for each of the pool's blocks, whichever are fewer.
- *               b2p_paged_prefill_fp8_scratch_size() is enough for a pool of any size. Calls of few
- *               query tiles cut the keys into runs by the table's width: tables no wider than
- *               their longest history serve them best.
+ *               The copy has a block for each table entry or for each of the num_slots / block_size
+ *               blocks of the pool, whichever are fewer. b2p_paged_prefill_fp8_scratch_size() is
+ *               enough for a pool of any size.
+ *   table_width : entries of a table row that count, block_table_stride at most (and that much in
+ *               b2p_paged_prefill_fp8): an upper bound of ceil(context / block_size). A longer
+ *               context is cut to it and sets B2P_DEV_BLOCK_RANGE, or is attended all the same. Calls
+ *               of few query tiles cut the keys into runs by it, so a wide bound on short histories
+ *               costs time (four whole prompts of 512 tokens: 61.6 us with 256 entries, 27.5 with 32).
  */
 B2P_API size_t b2p_paged_prefill_fp8_pool_scratch_size(int num_seqs, int64_t total_q,
                  int64_t table_width, int64_t num_slots, int num_q_heads, int num_kv_heads,
@@ -373,6 +376,16 @@ B2P_API int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_t q
                  const void* key_cache, const void* value_cache, const float* key_scales,
                  const float* value_scales, int64_t layer_index, int64_t num_layers,
                  int64_t num_slots, const int32_t* block_tables, int64_t block_table_stride,
+                 const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
+                 int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
+                 int block_size, float scale, void* out, int64_t out_tok_stride,
+                 int64_t out_head_stride, void* workspace, size_t workspace_size, void* scratch,
+                 size_t scratch_size, int dtype,
+                 int32_t* err_flag, void* stream);
+B2P_API int b2p_paged_prefill_fp8_reach(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                 const void* key_cache, const void* value_cache, const float* key_scales,
+                 const float* value_scales, int64_t layer_index, int64_t num_layers,
+                 int64_t num_slots, const int32_t* block_tables, int64_t block_table_stride, int64_t table_width,
                  const int32_t* cu_seqlens_q, const int32_t* context_lens, int num_seqs,
                  int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
                  int block_size, float scale, void* out, int64_t out_tok_stride,

@@ -54,6 +54,7 @@ EXPORTED_SYMBOLS = (
     "b2p_paged_prefill_fp8_scratch_size",
     "b2p_paged_prefill_fp8_pool_scratch_size",
     "b2p_paged_prefill_fp8",
+    "b2p_paged_prefill_fp8_reach",
     "b2p_verify_drafts",
     "b2p_verify_drafts_greedy",
     "b2p_copy_blocks",
@@ -136,6 +137,11 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "b2p_paged_prefill_fp8": (
         _i32,
         [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _i32, _i64, _i32,
+         _i32, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _sz, _p, _sz, _i32, _p, _p],
+    ),
+    "b2p_paged_prefill_fp8_reach": (
+        _i32,
+        [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i32, _i64, _i32,
          _i32, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _sz, _p, _sz, _i32, _p, _p],
     ),
     "b2p_verify_drafts": (

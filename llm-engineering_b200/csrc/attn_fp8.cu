@@ -271,7 +271,7 @@ Scratch scratch_of(int num_seqs, int64_t width, int64_t pool_blocks, int num_kv_
 // Runs that every (query tile, pair of heads) item's keys are cut into, where a call has too few
 // items for the SMs: one wave of them where they are fewer than half the SMs, else about three
 // per SM, so that a long history next to short ones does not set the time. A run is at least
-// kRunTiles KV tiles of the longest history that the block tables can hold. Four 512-token
+// kRunTiles KV tiles of the longest history that table_width allows (for the lengths are on the device). Four 512-token
 // slices over 100 to 7777 tokens (14/2 heads): 103 us whole, 88 in two runs, 78 in three, 89 in
 // six; one such slice over 8000 tokens (12/2 heads): 63 in five runs, 83 in eight (a second
 // wave); four whole 512-token prompts: 47 whole, 60 in four runs.
@@ -374,21 +374,23 @@ extern "C" size_t b2p_paged_prefill_fp8_scratch_size(int num_seqs, int64_t total
                                                  head_dim, block_size, max_q_len, dtype);
 }
 
-extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
-                                     const void* key_cache, const void* value_cache,
-                                     const float* key_scales, const float* value_scales,
-                                     int64_t layer_index, int64_t num_layers, int64_t num_slots,
-                                     const int32_t* block_tables, int64_t block_table_stride,
-                                     const int32_t* cu_seqlens_q, const int32_t* context_lens,
-                                     int num_seqs, int64_t total_q, int max_q_len, int num_q_heads,
-                                     int num_kv_heads, int head_dim, int block_size, float scale,
-                                     void* out, int64_t out_tok_stride, int64_t out_head_stride,
-                                     void* workspace, size_t workspace_size, void* scratch,
-                                     size_t scratch_size, int dtype,
-                                     int32_t* err_flag, void* stream) {
+extern "C" int b2p_paged_prefill_fp8_reach(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                           const void* key_cache, const void* value_cache,
+                                           const float* key_scales, const float* value_scales,
+                                           int64_t layer_index, int64_t num_layers, int64_t num_slots,
+                                           const int32_t* block_tables, int64_t block_table_stride,
+                                           int64_t table_width,
+                                           const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                                           int num_seqs, int64_t total_q, int max_q_len, int num_q_heads,
+                                           int num_kv_heads, int head_dim, int block_size, float scale,
+                                           void* out, int64_t out_tok_stride, int64_t out_head_stride,
+                                           void* workspace, size_t workspace_size, void* scratch,
+                                           size_t scratch_size, int dtype,
+                                           int32_t* err_flag, void* stream) {
   const int rc = check_args(key_cache, value_cache, workspace, scale, layer_index, num_layers, num_slots, num_seqs, total_q, max_q_len,
                             num_q_heads, num_kv_heads, head_dim, block_size, block_table_stride,
                             dtype);
+  if (rc == B2P_OK && (table_width < 0 || table_width > block_table_stride)) return B2P_EINVAL;
   if (rc != B2P_OK || num_seqs == 0 || total_q == 0 || max_q_len == 0) return rc;
   if (!q || !key_cache || !value_cache || !key_scales || !value_scales || !block_tables ||
       !cu_seqlens_q || !context_lens || !out)
@@ -401,7 +403,7 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
                         max_q_len, num_q_heads, num_kv_heads, head_dim, block_size, scale, out,
                         out_tok_stride, out_head_stride, workspace, workspace_size, dtype,
                         err_flag, stream);
-  const int64_t width = block_table_stride;
+  const int64_t width = table_width;
   if (tile_shape(head_dim, block_size, dtype) && aligned(key_cache, 16) && aligned(value_cache, 16) && width > 0 &&
       tile_rows_fit(q, q_tok_stride, q_head_stride, out, out_tok_stride, out_head_stride)) {
     const int splits = key_splits(num_seqs, total_q, width, num_q_heads, num_kv_heads, block_size);
@@ -461,9 +463,9 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
     if (wrc != B2P_OK) return wrc;
     const int trc = b2p_prefill_tc_runs(
         q, q_tok_stride, q_head_stride, w.wide[0], w.wide[1], need.blocks * block_size,
-        need.own_ids ? block_tables : w.tables, width, w.safe_cu, w.safe_ctx, num_seqs, total_q, num_q_heads,
-        num_kv_heads, head_dim, block_size, scale, out, out_tok_stride, out_head_stride, dtype, err_flag, stream,
-        w.claims, splits, part, w.lse);
+        need.own_ids ? block_tables : w.tables, need.own_ids ? block_table_stride : width, w.safe_cu, w.safe_ctx,
+        num_seqs, total_q, num_q_heads, num_kv_heads, head_dim, block_size, scale, out, out_tok_stride,
+        out_head_stride, dtype, err_flag, stream, w.claims, splits, part, w.lse);
     if (trc != B2P_EUNSUPPORTED) return trc;  // a device that the tile kernel does not fit: as b2p_paged_prefill does
   }
   if (dtype != B2P_F32) b2p_host::note_fallback(3);
@@ -472,4 +474,24 @@ extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_
                            cu_seqlens_q, context_lens, num_seqs, total_q, num_q_heads,
                            num_kv_heads, head_dim, block_size, scale, out, out_tok_stride,
                            out_head_stride, dtype, err_flag, stream);
+}
+
+// The same over tables whose whole width counts.
+extern "C" int b2p_paged_prefill_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                     const void* key_cache, const void* value_cache,
+                                     const float* key_scales, const float* value_scales,
+                                     int64_t layer_index, int64_t num_layers, int64_t num_slots,
+                                     const int32_t* block_tables, int64_t block_table_stride,
+                                     const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                                     int num_seqs, int64_t total_q, int max_q_len, int num_q_heads,
+                                     int num_kv_heads, int head_dim, int block_size, float scale,
+                                     void* out, int64_t out_tok_stride, int64_t out_head_stride,
+                                     void* workspace, size_t workspace_size, void* scratch,
+                                     size_t scratch_size, int dtype,
+                                     int32_t* err_flag, void* stream) {
+  return b2p_paged_prefill_fp8_reach(
+      q, q_tok_stride, q_head_stride, key_cache, value_cache, key_scales, value_scales, layer_index, num_layers,
+      num_slots, block_tables, block_table_stride, block_table_stride, cu_seqlens_q, context_lens, num_seqs, total_q,
+      max_q_len, num_q_heads, num_kv_heads, head_dim, block_size, scale, out, out_tok_stride, out_head_stride,
+      workspace, workspace_size, scratch, scratch_size, dtype, err_flag, stream);
 }

@@ -647,6 +647,7 @@ def paged_prefill_fp8(
     out: torch.Tensor | None = None,
     workspace: torch.Tensor | None = None,
     err_flag: torch.Tensor | None = None,
+    max_context: int | None = None,
 ) -> torch.Tensor:
     """K3 over the 8-bit cache: packed variable-length causal attention over the paged history
     (the rows of drafted tokens, of prompt slices or of whole prompts).
@@ -657,8 +658,9 @@ def paged_prefill_fp8(
     owns are left alone in out. Calls of many rows widen the histories into a 16-bit copy, allocated
     for the call, of one layer's blocks: ``num_seqs * block_tables.shape[1]`` of them or as many as the
     pool has, whichever are fewer (with fp32 partial results where few query tiles are spread over
-    the SMs by their keys, in runs sized by the tables' width: pass tables no wider than the
-    longest history). The copy is in q's type: with f16 queries over a pool that bf16 or fp32 rows
+    the SMs by their keys). ``max_context`` bounds the context_lens where the tables are wider than
+    those need: the runs of keys are sized by it, else by the tables' width (a longer context is cut
+    and flagged, or attended all the same). The copy is in q's type: with f16 queries over a pool that bf16 or fp32 rows
     went into, values past 65,536 are flagged (B2P_DEV_VALUE_RANGE) and cut.
     """
     index, (layers, slots, hkv, d) = _check_fp8_pool(key_cache, value_cache, key_scales,
@@ -669,14 +671,19 @@ def paged_prefill_fp8(
     _vector(index, "cu_seqlens_q", cu_seqlens_q, torch.int32)
     width = _check_tables(index, n, block_tables, context_lens)
     workspace = _fp8_workspace(index, workspace, n, hq, hkv, d, max_q_len)
+    reach = width
+    if max_context is not None:
+        if max_context < 0:
+            raise ValueError("max_context must not be negative")
+        reach = min(width, max(1, -(-max_context // block_size)))
     scratch, size = None, 0
     if max_q_len * hq > _row_columns() * hkv:
         size = _lib.load().b2p_paged_prefill_fp8_pool_scratch_size(
-            n, total_q, width, slots, hq, hkv, d, block_size, max_q_len, code)
+            n, total_q, reach, slots, hq, hkv, d, block_size, max_q_len, code)
         scratch = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _call("b2p_paged_prefill_fp8", index, q.data_ptr(), qt, qh, key_cache.data_ptr(),
+    _call("b2p_paged_prefill_fp8_reach", index, q.data_ptr(), qt, qh, key_cache.data_ptr(),
           value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), layer_index,
-          layers, slots, block_tables.data_ptr(), width, cu_seqlens_q.data_ptr(),
+          layers, slots, block_tables.data_ptr(), width, reach, cu_seqlens_q.data_ptr(),
           context_lens.data_ptr(), n, total_q, max_q_len, hq, hkv, d, block_size, scale,
           out.data_ptr(), ot, oh, workspace.data_ptr(), workspace.numel(), _ptr(scratch), size,
           code, _err_flag(index, err_flag))

@@ -84,9 +84,10 @@ class StepBatch:
     # the cache hook, since a block's scale depends on every row in it.
     key_scales: torch.Tensor | None = None
     value_scales: torch.Tensor | None = None
-    # The prefill executions' block tables for an 8-bit pool, as wide as those need: the call sizes
-    # its scratch and its runs of keys by the width, and decode rows' histories may be far longer.
-    prefill_tables: torch.Tensor | None = None
+    # The longest prefill execution's context: attention over an 8-bit pool sizes its scratch and its
+    # runs of keys by it, and decode rows' histories, which the tables are wide enough for, may be
+    # far longer.
+    prefill_context: int = 0
 
 
 def _phase_of(execution) -> str:
@@ -126,9 +127,10 @@ def paged_attention(module: torch.nn.Module, query: torch.Tensor, key: torch.Ten
                                batch.block_size, scaling, out=out[:nd],
                                workspace=batch.workspace, err_flag=batch.err)
         if nd < batch.num_execs:
-            k.paged_prefill_fp8(q, *pool, batch.prefill_tables, batch.cu_seqlens_q[nd:],
+            k.paged_prefill_fp8(q, *pool, batch.block_tables[nd:], batch.cu_seqlens_q[nd:],
                                 batch.context_lens[nd:], batch.max_q_len, batch.block_size,
-                                scaling, out=out, workspace=batch.workspace, err_flag=batch.err)
+                                scaling, out=out, workspace=batch.workspace, err_flag=batch.err,
+                                max_context=batch.prefill_context)
         return out.unsqueeze(0), None
     if nd and batch.fused_decode:
         k.paged_decode_append(q[:nd], key[0].transpose(0, 1)[:nd], value[0].transpose(0, 1)[:nd],
@@ -414,13 +416,9 @@ class B200PagedModelRunner:
             tables = dev_i32[3 * n:].view(n, width)
             md = kernels.build_metadata(qlens, ctx, rows, tables, bs, total_q, 0, self._err)
         key_scales = getattr(self._storage, "key_scales", None)
-        prefill_tables = None
         if key_scales is not None:
             if d["block_size"] != self._storage.block_size:
                 raise ValueError("an 8-bit cache needs block-structured slot_ids")
-            if num_decode < n:
-                reach = max(-(-length // bs) for length in d["lengths"][num_decode:])
-                prefill_tables = tables[num_decode:, :reach].contiguous()
             need = kernels.fp8_workspace_size(n, self._hq, self._hkv, self._head_dim)
         else:
             need = kernels.decode_workspace_size(max(num_decode, 1), self._hq, self._hkv,
@@ -437,7 +435,7 @@ class B200PagedModelRunner:
             fused_decode=(key_scales is None and num_decode > 0
                           and hasattr(kernels, "paged_decode_append")),
             key_scales=key_scales, value_scales=getattr(self._storage, "value_scales", None),
-            prefill_tables=prefill_tables)
+            prefill_context=max(d["lengths"][num_decode:], default=0))
         return batch, input_ids
 
     # ------------------------------------------------------------------ ModelRunner

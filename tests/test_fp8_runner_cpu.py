@@ -30,8 +30,9 @@ class Notes(CpuKernels):
         self.decode.append((bt.clone(), ctx.tolist(), bt.is_contiguous()))
         return out.zero_()
 
-    def paged_prefill_fp8(self, q, kc, vc, ks, vs, layer, bt, cu, ctx, max_q, bs, scale, out=None, **kw):
-        self.prefill.append((bt.clone(), cu.tolist(), ctx.tolist(), bt.is_contiguous()))
+    def paged_prefill_fp8(self, q, kc, vc, ks, vs, layer, bt, cu, ctx, max_q, bs, scale, out=None,
+                          max_context=None, **kw):
+        self.prefill.append((bt.clone(), cu.tolist(), ctx.tolist(), bt.is_contiguous(), max_context))
         return out
 
 
@@ -46,7 +47,7 @@ class Execution:
 
 @pytest.mark.parametrize("decode", [[], [90], [5, 64]])
 @pytest.mark.parametrize("prompts", [[(20, 20)], [(40, 8), (17, 17), (3, 2)]])
-def test_prompts_get_tables_as_wide_as_they_need(monkeypatch, decode, prompts):
+def test_prompts_are_bounded_by_their_own_contexts(monkeypatch, decode, prompts):
     notes = Notes()
     monkeypatch.setattr(runner_mod, "_ops", notes)
     model = tiny_model()
@@ -59,9 +60,8 @@ def test_prompts_get_tables_as_wide_as_they_need(monkeypatch, decode, prompts):
     runner.forward([Execution(f"r{i}", n, q, b) for i, (n, q, b) in enumerate(zip(lengths, q_lens, blocks))])
     nd = len(decode)
     assert len(notes.prefill) == 2 and len(notes.decode) == (2 if nd else 0)  # one per layer
-    width = max(len(b) for b in blocks[nd:])
-    for table, cu, ctx, contiguous in notes.prefill:
-        assert table.shape == (len(prompts), width) and contiguous
+    for table, cu, ctx, contiguous, bound in notes.prefill:
+        assert bound == max(lengths[nd:]) and contiguous and len(table) == len(prompts)
         assert [row[:len(b)].tolist() for row, b in zip(table, blocks[nd:])] == blocks[nd:]
         assert ctx == lengths[nd:] and cu[0] == nd and cu[-1] == sum(q_lens)
     for table, ctx, contiguous in notes.decode:

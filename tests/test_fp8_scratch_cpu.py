@@ -43,3 +43,19 @@ def test_calls_that_need_none():
     assert c.b2p_paged_prefill_fp8_pool_scratch_size(2, 300, 10, 640, 4, 2, 64, 16, 200, 2) == 0  # fp32
     assert c.b2p_paged_prefill_fp8_pool_scratch_size(2, 300, 10, 640, 4, 2, 40, 16, 200, 0) == 0  # head_dim
     assert c.b2p_paged_prefill_fp8_pool_scratch_size(2, 300, 10, 0, 4, 2, 64, 16, 200, 0) == 0
+
+
+def test_refusals_of_a_width():
+    from llm_engineering_b200 import _lib
+
+    c = lib()
+    fake = 1 << 20
+
+    def prefill(width, stride=4, n=1, rows=200):
+        return c.b2p_paged_prefill_fp8_reach(fake, 256, 64, fake, fake, fake, fake, 0, 1, 64, fake, stride, width, fake,
+                                             fake, n, rows, 200, 4, 2, 64, 16, 0.1, fake, 256, 64, None, 0, None, 0, 0,
+                                             None, None)
+
+    assert prefill(5) == prefill(-1) == _lib.B2P_EINVAL
+    assert prefill(4, n=0) == prefill(0, rows=0) == _lib.B2P_OK
+    assert prefill(4) == prefill(1) == _lib.B2P_EWORKSPACE

@@ -100,3 +100,39 @@ def test_what_a_call_allocates_follows_the_pool(ops):
     taken = torch.cuda.max_memory_allocated() - before
     # K and V of the pool in 16 bits, and the partial results of at most eight runs
     assert taken <= 2 * blocks * bs * hkv * d * 2 + 8 * q.numel() * 4 * (1 + 1 / d) + (1 << 20)
+
+
+@pytest.mark.parametrize("q_lens,past", [([200, 90, 300], [40, 0, 513]), ([130], [2300]), ([5, 3], [90, 7])])
+def test_a_bound_on_the_contexts(ops, q_lens, past):
+    """Wide tables with a bound: the narrow tables' results, bit for bit, and their scratch. A context
+    past the bound is cut to the blocks that the bound covers, and flagged, in the many-row form."""
+    hq, hkv, d, bs = 12, 2, 128, 16
+    rng = np.random.default_rng(len(q_lens))
+    ctx = [a + b for a, b in zip(past, q_lens)]
+    tables, bt, blocks = tables_for(rng, ctx, bs, spare=4000)
+    pool = Pool(rng, 1, blocks, bs, hkv, d)
+    dev = pool.device()
+    q = torch.from_numpy(rng.standard_normal((sum(q_lens), hq, d))).to(torch.bfloat16).cuda()
+    cu = i32([0, *np.cumsum(q_lens)])
+    ws = ops.make_fp8_workspace(len(ctx), hq, hkv, d, torch.device("cuda"), max(q_lens))
+
+    def call(table, **kw):
+        err, out = i32([0]), torch.empty_like(q)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        ops.paged_prefill_fp8(q, *dev, 0, table, cu, i32(ctx), max(q_lens), bs, d ** -0.5, out=out, workspace=ws,
+                              err_flag=err, **kw)
+        taken = torch.cuda.max_memory_allocated() - before
+        return out, err.item(), taken
+
+    narrow, flag, least = call(bt.cuda())
+    assert flag == 0
+    for bound in (max(ctx), bt.shape[1] * bs):
+        got, flag, taken = call(widened(bt, 1000).cuda(), max_context=bound)
+        assert torch.equal(got, narrow) and taken <= least + (1 << 16) and flag == 0
+    if max(q_lens) > 5:
+        got, flag, _ = call(widened(bt, 1000).cuda(), max_context=max(ctx) - 20)
+        assert flag == 2
+    with pytest.raises(ValueError, match="max_context"):
+        call(bt.cuda(), max_context=-1)
